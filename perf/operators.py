@@ -19,8 +19,9 @@ own = False
 
 GROUP = 32
 DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
-# smallest and largest e: a scale stays a normal number, and values packed from f16 stay f16 numbers
-E_RANGE = {"bf16": (-126, 127), "f32": (-126, 127), "f16": (-24, 9)}
+# smallest and largest e: a scale stays a normal number, values packed from f16 stay f16 numbers, and 127 * 2^e
+# stays below the type's largest number
+E_RANGE = {"bf16": (-126, 121), "f32": (-126, 121), "f16": (-24, 9)}
 
 
 def listed():
