@@ -116,6 +116,72 @@ int sm_stats_accumulate_noalloc(const void* rows, int dtype, int64_t n_rows, int
                                 int64_t row_stride, int64_t col_stride, float* sum_sq, float* sum,
                                 void* stream);
 
+/* ------------------------------------------- 8-bit activation checkpoints
+ * A layer's input held for the backward pass in 8 bits (no counterpart in the
+ * reference).  x [rows, cols] is kept as
+ *   values    int8  [rows, ld]   ld  = SM_ACTIVATION_LD(cols), padding 0
+ *   exponents uint8 [rows, lde]  lde = SM_ACTIVATION_LDE(cols), padding 127
+ * in groups of SM_ACTIVATION_GROUP consecutive columns of a row:
+ *   e = the smallest integer with max|x| <= 127 * 2^e, stored as e + 127
+ *   q = rint(x * 2^-e) (ties to even), and x^ = q * 2^e stands for x
+ * so |x - x^| <= 2^(e-1).  e is clamped to [-126, 121], or [-24, 9] for an F16
+ * input, so that x^ is finite (|x| > 127 * 2^121, or 65024 in F16, is held as
+ * that, less than 2^e away).  A group with a non-finite
+ * member has exponent code 255, values 0, and stands for NaN.
+ * `values` and `exponents` must be 16- and 4-byte aligned. */
+#define SM_ACTIVATION_GROUP 32
+#define SM_ACTIVATION_LD(cols) (((int64_t)(cols) + 15) / 16 * 16)
+#define SM_ACTIVATION_LDE(cols) (((int64_t)(cols) + 127) / 128 * 4)
+
+/* Bytes of workspace sm_activation_pack and sm_gelu_forward need when they
+ * return column sums of an [n_rows, n_cols] tensor. */
+size_t sm_activation_sums_workspace_bytes(int64_t n_rows, int64_t n_cols);
+
+/* Packs x (F32 / BF16 / F16, x[r, c] at x + (r * row_stride + c * col_stride)
+ * elements) and, with sums != NULL, writes sums[0, c] = sum_r x^2 and
+ * sums[1, c] = sum_r x (float [2, n_cols]) from the same read of x: what
+ * sm_stats_accumulate adds for the forward hook.  Deterministic. */
+int sm_activation_pack(const void* x, int dtype, int64_t n_rows, int64_t n_cols, int64_t row_stride,
+                       int64_t col_stride, int8_t* values, uint8_t* exponents, float* sums, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* out [n_rows, n_cols] (contiguous, F32 / BF16 / F16) = x^.  Exact in F32 and
+ * BF16, and in F16 where the checkpoint was packed from F16. */
+int sm_activation_unpack(const int8_t* values, const uint8_t* exponents, int64_t n_rows, int64_t n_cols, void* out,
+                         int dtype, void* stream);
+
+/* GELU forms */
+#define SM_GELU_ERF 0   /* x * Phi(x) */
+#define SM_GELU_TANH 1  /* 0.5 x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) */
+
+/* y = gelu(x) (contiguous, x's type).  in_values / in_exponents (NULL: not
+ * kept) receive the checkpoint of x that sm_gelu_backward reads; out_values /
+ * out_exponents (NULL: not kept) that of the rounded y, with y's column sums
+ * in sums (NULL: not wanted; needs out_values). */
+int sm_gelu_forward(const void* x, int dtype, int64_t n_rows, int64_t n_cols, int64_t row_stride,
+                    int64_t col_stride, int form, void* y, int8_t* in_values, uint8_t* in_exponents,
+                    int8_t* out_values, uint8_t* out_exponents, float* sums, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* dx = delta * gelu'(x^) (contiguous, delta's type; delta of any strides). */
+int sm_gelu_backward(const void* delta, int dtype, int64_t n_rows, int64_t n_cols, int64_t row_stride,
+                     int64_t col_stride, const int8_t* values, const uint8_t* exponents, int form, void* dx,
+                     void* stream);
+
+/* Bytes of workspace sm_weight_gradient needs for the same arguments. */
+size_t sm_weight_gradient_workspace_bytes(const void* delta, int dtype, int64_t n_rows, int64_t d_out,
+                                          int64_t row_stride, int64_t col_stride, int64_t d_in);
+
+/* Weight gradient of a linear layer from its packed input:
+ *   out[o, i] = sum_t delta[t, o] * x^[t, i]     (contiguous [d_out, d_in])
+ * delta [n_rows, d_out] F32 / BF16 / F16 of any strides; the checkpoint is of
+ * an [n_rows, d_in] input, packed from F16 if delta is F16.  Products are
+ * exact and summed in FP32 on the tensor cores in an order that depends on the
+ * sizes alone; out (F32 / BF16 / F16) is rounded once. */
+int sm_weight_gradient(const void* delta, int dtype, int64_t n_rows, int64_t d_out, int64_t row_stride,
+                       int64_t col_stride, const int8_t* values, const uint8_t* exponents, int64_t d_in, void* out,
+                       int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------ optimizer plan */
 
 /* One selected weight matrix (a torch Linear weight, shape [d_out, d_in],

@@ -32,6 +32,8 @@ SM_GEMM_B_KMAJOR = 1
 SM_GEMM_A_MNMAJOR = 2
 SM_GEMM_PAIR = 4
 SM_GEMM_BN128 = 8
+SM_GELU_ERF = 0
+SM_GELU_TANH = 1
 SM_EXPORT_WEIGHTS = 0
 SM_EXPORT_BF16_DELTA = 1
 SM_TCLASS_GEMM = 0
@@ -95,6 +97,17 @@ SIGNATURES = {
                                      _c_void_p, _c_size, _c_void_p]),
     "sm_stats_accumulate_noalloc": (_c_int, [_c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_void_p,
                                              _c_void_p, _c_void_p]),
+    "sm_activation_sums_workspace_bytes": (_c_size, [_c_i64, _c_i64]),
+    "sm_activation_pack": (_c_int, [_c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_void_p, _c_void_p,
+                                    _c_void_p, _c_void_p, _c_size, _c_void_p]),
+    "sm_activation_unpack": (_c_int, [_c_void_p, _c_void_p, _c_i64, _c_i64, _c_void_p, _c_int, _c_void_p]),
+    "sm_gelu_forward": (_c_int, [_c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_void_p, _c_void_p,
+                                 _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_size, _c_void_p]),
+    "sm_gelu_backward": (_c_int, [_c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_void_p, _c_void_p, _c_int,
+                                  _c_void_p, _c_void_p]),
+    "sm_weight_gradient_workspace_bytes": (_c_size, [_c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64]),
+    "sm_weight_gradient": (_c_int, [_c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_void_p, _c_void_p, _c_i64,
+                                    _c_void_p, _c_int, _c_void_p, _c_size, _c_void_p]),
     "sm_plan_workspace_bytes": (_c_int, [ctypes.POINTER(SmPlanSpec), ctypes.POINTER(_c_size)]),
     "sm_plan_create": (_c_int, [ctypes.POINTER(SmPlanSpec), _c_void_p, _c_size, _c_void_p, ctypes.POINTER(_c_void_p)]),
     "sm_plan_step": (_c_int, [_c_void_p, ctypes.POINTER(SmStepArgs), _c_void_p]),

@@ -20,6 +20,7 @@ LIB_NAME = "libsandmuon_b200.so"
 LIB_PATH = PACKAGE / LIB_NAME
 SOURCES = [CSRC / "libsandmuon_b200.cu"]
 DEPENDS = SOURCES + [CSRC / "sm_common.cuh", CSRC / "sm_gemm.cuh", CSRC / "sm_kernels.cuh",
+                     CSRC / "sm_activation.cuh", CSRC / "sm_wgrad.cuh", CSRC / "sm_activation_host.cuh",
                      ROOT / "include" / "sandmuon_b200.h"]
 
 NVCC_FLAGS = [

@@ -32,6 +32,7 @@
 #include "sm_common.cuh"
 #include "sm_gemm.cuh"
 #include "sm_kernels.cuh"
+#include "sm_wgrad.cuh"
 
 namespace smb {
 
@@ -2491,3 +2492,5 @@ int sm_ipc_close(void* base) {
 }
 
 }  // extern "C"
+
+#include "sm_activation_host.cuh"
