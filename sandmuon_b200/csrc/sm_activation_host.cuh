@@ -161,8 +161,8 @@ struct WgradGeometry {
   int planes, bk;
   int64_t plane_ld;    // elements
   int64_t tiles_m, tiles_n, kblocks;
-  int workers;
-  bool partial;        // some tile is shared by workers
+  int workers, shared, parts;  // see WgradArgs
+  bool partial;        // some tile is held by several workers
   size_t plane_bytes, partial_bytes;
 };
 
@@ -180,10 +180,24 @@ static int wgrad_geometry(const void* delta, int dtype, int64_t rows, int64_t d_
   g->tiles_m = cdiv(d_out, kWgTileM);
   g->tiles_n = cdiv(d_in, kWgTileN);
   g->kblocks = cdiv(rows, g->bk);
-  const int64_t total = g->tiles_m * g->tiles_n * g->kblocks;
-  g->workers = static_cast<int>(std::min<int64_t>(pairs, cdiv(total, kWgMinTokens / g->bk)));
+  const int64_t tiles = g->tiles_m * g->tiles_n;
+  if (tiles > INT32_MAX / 2) return fail(SM_ERR_ARG, "too many output tiles");
+  g->shared = static_cast<int>(tiles % pairs);
+  g->parts = 0;
+  const int64_t least = kWgMinTokens / g->bk;  // k-blocks of a share
+  g->workers = tiles >= pairs ? pairs : static_cast<int>(std::min<int64_t>(pairs, cdiv(tiles * g->kblocks, least)));
+  if (g->shared > 0 && tiles < pairs) {
+    // Equal parts of each tile leave workers idle but give each worker one
+    // tile; stretches across tiles keep all busy but cost most workers a
+    // second epilogue, about kWgEpilogueBlocks k-blocks of time.
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(g->workers / tiles, g->kblocks / least));
+    const int64_t even = cdiv(g->kblocks, parts);
+    const int64_t across = cdiv(tiles * g->kblocks, g->workers) + kWgEpilogueBlocks;
+    if (even <= across) g->parts = static_cast<int>(parts), g->workers = static_cast<int>(tiles * parts);
+  }
   g->partial = false;
-  for (int w = 1; w < g->workers && !g->partial; ++w) g->partial = wgrad_begin(total, g->workers, w) % g->kblocks != 0;
+  for (int w = 1; w < g->workers && !g->partial; ++w)
+    g->partial = wgrad_begin(g->shared, g->parts, static_cast<int>(g->kblocks), g->workers, w) % g->kblocks != 0;
   g->plane_bytes = g->direct ? 0 : round_up(static_cast<int64_t>(g->planes) * rows * g->plane_ld * 2, 256);
   g->partial_bytes = g->partial ? static_cast<size_t>(2 * g->workers) * kWgPartialFloats * sizeof(float) : 0;
   return SM_OK;
@@ -208,8 +222,7 @@ static int wgrad_launch(const WgradArgs& p, bool partial, cudaStream_t st) {
   SM_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
   if (!partial) return SM_OK;
   PdlScope pdl(true);
-  const unsigned tiles = static_cast<unsigned>(p.total / p.kblocks);
-  return launch_kernel(k_wgrad_join<OUT>, dim3(tiles, 16), dim3(128), 0, st, p);
+  return launch_kernel(k_wgrad_join<OUT>, dim3(static_cast<unsigned>(p.shared), 64), dim3(256), 0, st, p);
 }
 
 template <int PLANES, bool F16, int BK>
@@ -370,7 +383,6 @@ int sm_weight_gradient(const void* delta, int dtype, int64_t n_rows, int64_t d_o
   if (g.plane_bytes + g.partial_bytes > 0 &&
       (workspace == nullptr || !aligned(workspace, 256) || workspace_bytes < g.plane_bytes + g.partial_bytes))
     return fail(SM_ERR_WORKSPACE, "weight gradient workspace too small or not 256-byte aligned");
-  if (g.tiles_m * g.tiles_n > INT32_MAX) return fail(SM_ERR_ARG, "too many output tiles");
   WgradArgs p;
   memset(&p, 0, sizeof(p));
   const int64_t plane_elems = n_rows * g.plane_ld;
@@ -399,10 +411,12 @@ int sm_weight_gradient(const void* delta, int dtype, int64_t n_rows, int64_t d_o
   p.rows = static_cast<int>(n_rows);
   p.d_out = static_cast<int>(d_out);
   p.d_in = static_cast<int>(d_in);
+  p.tiles = static_cast<int>(g.tiles_m * g.tiles_n);
   p.tiles_n = static_cast<int>(g.tiles_n);
   p.kblocks = static_cast<int>(g.kblocks);
-  p.total = g.tiles_m * g.tiles_n * g.kblocks;
   p.workers = g.workers;
+  p.shared = g.shared;
+  p.parts = g.parts;
   p.out = out;
   p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + g.plane_bytes);
   p.vec_out = aligned(out, 16) && (d_in * elem_size(out_dtype)) % 16 == 0;
