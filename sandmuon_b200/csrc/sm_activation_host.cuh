@@ -166,6 +166,17 @@ struct WgradGeometry {
   size_t plane_bytes, partial_bytes;
 };
 
+static void wgrad_shares(const WgradGeometry& g, WgradArgs* p) {
+  p->tiles = static_cast<int>(g.tiles_m * g.tiles_n);
+  p->tiles_n = static_cast<int>(g.tiles_n);
+  p->kblocks = static_cast<int>(g.kblocks);
+  p->workers = g.workers;
+  p->shared = g.shared;
+  p->parts = g.parts;
+  p->each = g.parts > 0 ? 0 : p->shared * p->kblocks / g.workers;
+  p->more = g.parts > 0 ? 0 : p->shared * p->kblocks % g.workers;
+}
+
 static int wgrad_geometry(const void* delta, int dtype, int64_t rows, int64_t d_out, int64_t rs, int64_t cs,
                           int64_t d_in, WgradGeometry* g) {
   DeviceInfo* di;
@@ -195,9 +206,13 @@ static int wgrad_geometry(const void* delta, int dtype, int64_t rows, int64_t d_
     const int64_t across = cdiv(tiles * g->kblocks, g->workers) + kWgEpilogueBlocks;
     if (even <= across) g->parts = static_cast<int>(parts), g->workers = static_cast<int>(tiles * parts);
   }
+  // WgradArgs counts k-blocks in 32 bits
+  if (g->kblocks * std::max(pairs, g->workers) > INT32_MAX)
+    return fail(SM_ERR_ARG, "too many rows for a weight gradient");
+  WgradArgs p;
+  wgrad_shares(*g, &p);
   g->partial = false;
-  for (int w = 1; w < g->workers && !g->partial; ++w)
-    g->partial = wgrad_begin(g->shared, g->parts, static_cast<int>(g->kblocks), g->workers, w) % g->kblocks != 0;
+  for (int w = 1; w < g->workers && !g->partial; ++w) g->partial = wgrad_begin(p, w) % p.kblocks != 0;
   g->plane_bytes = g->direct ? 0 : round_up(static_cast<int64_t>(g->planes) * rows * g->plane_ld * 2, 256);
   g->partial_bytes = g->partial ? static_cast<size_t>(2 * g->workers) * kWgPartialFloats * sizeof(float) : 0;
   return SM_OK;
@@ -411,12 +426,7 @@ int sm_weight_gradient(const void* delta, int dtype, int64_t n_rows, int64_t d_o
   p.rows = static_cast<int>(n_rows);
   p.d_out = static_cast<int>(d_out);
   p.d_in = static_cast<int>(d_in);
-  p.tiles = static_cast<int>(g.tiles_m * g.tiles_n);
-  p.tiles_n = static_cast<int>(g.tiles_n);
-  p.kblocks = static_cast<int>(g.kblocks);
-  p.workers = g.workers;
-  p.shared = g.shared;
-  p.parts = g.parts;
+  wgrad_shares(g, &p);
   p.out = out;
   p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + g.plane_bytes);
   p.vec_out = aligned(out, 16) && (d_in * elem_size(out_dtype)) % 16 == 0;

@@ -12,14 +12,14 @@
 // Both operands have the sum's axis t as their slow dimension, so both are
 // MN-major tiles (see Swz).  A CTA pair computes a 256 x 256 tile
 // (cta_group::2): each CTA stages 128 delta columns and 128 x^ columns.
-//   warp 0        producer: TMA loads of the delta tiles (128-byte swizzle,
-//                 counted on the leader's full barrier) and of the raw int8
-//                 tiles, and 4-byte asynchronous copies of their exponent codes
-//                 (both counted on this CTA's raw barrier)
+//   warp 0        delta producer: TMA loads (128-byte swizzle), counted on the
+//                 leader's barrier
 //   warp 1        MMA issuer (the leader's thread, for both CTAs)
 //   warps 2..9    epilogue: TMEM -> registers -> global
-//   warps 10..17  converters: raw int8 tile -> 16-bit x^ in the swizzled layout
-//                 the MMA reads, then an arrival on the leader's full barrier
+//   warps 10..25  converters: raw int8 tile -> 16-bit x^ in the swizzled layout
+//                 the MMA reads, then an arrival on the leader's barrier
+//   warp 26       raw producer: TMA loads of the int8 tiles and 4-byte
+//                 asynchronous copies of their exponent codes
 //
 // The tensor core's FP32 accumulation truncates, so its error grows with the
 // length of a chain of MMAs (7e-6 relative after 1024 steps of 16 tokens).  A
@@ -46,10 +46,12 @@
 namespace smb {
 
 constexpr int kWgTileM = 256, kWgTileN = 256;  // of a CTA pair
-constexpr int kWgConvWarps = 8;
+constexpr int kWgConvWarps = 16;
+constexpr int kWgConvGroups = 4;
 constexpr int kWgEpiWarps = 8;
 constexpr int kWgChain = 128;  // MMA steps summed by the tensor core alone
-constexpr int kWgThreads = 64 + 32 * (kWgEpiWarps + kWgConvWarps);
+constexpr int kWgRawWarp = 2 + kWgEpiWarps + kWgConvWarps;
+constexpr int kWgThreads = 32 * (kWgRawWarp + 1);
 constexpr int kWgPartialFloats = kWgTileM * kWgTileN;
 // k-blocks of one worker's share are at least this many (256 tokens), so that
 // a short sum is not cut into partial tiles that cost more than they save
@@ -73,79 +75,122 @@ struct WgradArgs {
   int workers;
   int shared;               // tiles 0 .. shared - 1 are shared out by k-blocks
   int parts;                // > 0: into this many equal parts, one per worker; 0: into
-                            // equal stretches of all workers, across tile borders
+                            // stretches of `each` k-blocks (`more` workers take one
+                            // more), across tile borders
+  int each, more;
   void* out;                // [d_out, d_in]
   float* partials;          // [2 * workers, kWgPartialFloats]
   int vec_out;              // rows of `out` take 16-byte stores
 };
 
-// First k-block (of the shared tiles, end to end) of worker w; w = workers
-// gives the end of the last worker's.
-__host__ __device__ inline int64_t wgrad_begin(int shared, int parts, int kblocks, int workers, int w) {
-  const int64_t total = static_cast<int64_t>(shared) * kblocks;
-  if (parts == 0) return total * w / workers;
-  return w >= shared * parts ? total
-                             : static_cast<int64_t>(w / parts) * kblocks + static_cast<int64_t>(kblocks) * (w % parts) / parts;
-}
-__device__ __forceinline__ int64_t wgrad_begin(const WgradArgs& p, int w) {
-  return wgrad_begin(p.shared, p.parts, p.kblocks, p.workers, w);
+// First k-block (counting through the shared tiles, end to end) of worker w,
+// w <= workers.  32 bits: the host keeps workers * kblocks below 2^31.
+__host__ __device__ inline int wgrad_begin(const WgradArgs& p, int w) {
+  if (p.parts == 0) return w * p.each + (w < p.more ? w : p.more);
+  if (w >= p.shared * p.parts) return p.shared * p.kblocks;
+  const int tile = w / p.parts;
+  return tile * p.kblocks + p.kblocks * (w - tile * p.parts) / p.parts;
 }
 
-// A worker's stretch of k-blocks inside one tile.
+// The worker that holds k-block b: the largest w with wgrad_begin(w) <= b.
+// b is the first or the last k-block of a tile.
+__host__ __device__ inline int wgrad_worker(const WgradArgs& p, int b) {
+  if (p.parts > 0) {
+    const int tile = b / p.kblocks;
+    return tile * p.parts + (b == tile * p.kblocks ? 0 : p.parts - 1);
+  }
+  const int big = p.more * (p.each + 1);
+  return b < big ? b / (p.each + 1) : p.more + (b - big) / p.each;
+}
+
+// A worker's stretch of k-blocks inside one tile, at tile row mi, column ni.
 struct WgSegment {
-  int tile, kb0, kb1;
+  int mi, ni, kb0, kb1;
 };
 
 // The segments of a worker: its share of the shared tiles, then whole tiles.
 struct WgIter {
-  int64_t pos, end;
-  int kblocks, index, tile, tiles, workers;
-  __device__ __forceinline__ WgIter(const WgradArgs& p, int worker)
-      : pos(wgrad_begin(p, worker)),
-        end(wgrad_begin(p, worker + 1)),
-        kblocks(p.kblocks),
-        index(0),
-        tile(p.shared + worker),
-        tiles(p.tiles),
-        workers(p.workers) {}
-  __device__ __forceinline__ bool valid() const { return pos < end || tile < tiles; }
+  int left, kb, tile, next_tile, index;
+  const WgradArgs& p;
+  __device__ __forceinline__ WgIter(const WgradArgs& args, int worker)
+      : next_tile(args.shared + worker), index(0), p(args) {
+    const int pos = wgrad_begin(p, worker);
+    left = wgrad_begin(p, worker + 1) - pos;
+    tile = pos / p.kblocks;
+    kb = pos - tile * p.kblocks;
+    skip();
+  }
+  __device__ __forceinline__ void skip() {
+    if (left == 0 && next_tile < p.tiles) {
+      tile = next_tile;
+      next_tile += p.workers;
+      kb = 0;
+      left = p.kblocks;
+    }
+  }
+  __device__ __forceinline__ bool valid() const { return left > 0; }
   __device__ __forceinline__ WgSegment get() const {
     WgSegment s;
-    if (pos < end) {
-      s.tile = static_cast<int>(pos / kblocks);
-      s.kb0 = static_cast<int>(pos - static_cast<int64_t>(s.tile) * kblocks);
-      s.kb1 = static_cast<int>(min(static_cast<int64_t>(kblocks), s.kb0 + (end - pos)));
-    } else {
-      s.tile = tile;
-      s.kb0 = 0;
-      s.kb1 = kblocks;
-    }
+    s.mi = tile / p.tiles_n;
+    s.ni = tile - s.mi * p.tiles_n;
+    s.kb0 = kb;
+    s.kb1 = min(p.kblocks, kb + left);
     return s;
   }
   __device__ __forceinline__ void next(const WgSegment& s) {
-    if (pos < end) {
-      pos += s.kb1 - s.kb0;
-      ++index;
-    } else {
-      tile += workers;
-    }
+    left -= s.kb1 - s.kb0;
+    ++tile;
+    kb = 0;
+    ++index;
+    skip();
   }
 };
 
+// Three rings, each as deep as its slots live long (measured in k-blocks of
+// about 0.3 us): delta tiles from their TMA load to the end of their MMAs
+// (about 2 us), raw tiles from their load to their conversion, converted tiles
+// from there to the end of the MMAs.  One ring of five whole stages instead
+// was bound by its depth: 512 us for 16384 x 2048 x 8192.
 template <int PLANES, int BK>
 struct WgSmem {
   static constexpr int kABytes = 128 * BK * 2;    // one plane of this CTA's delta columns
   static constexpr int kBBytes = 128 * BK * 2;    // this CTA's x^ columns
   static constexpr int kRawBytes = 128 * BK;
-  static constexpr int kStageBytes = PLANES * kABytes + kBBytes + kRawBytes;
   static constexpr int kCodeBytes = 4 * BK;       // exponent codes of a raw tile
+  static constexpr int kAStages = PLANES == 1 ? 6 : 5;
+  static constexpr int kBStages = 4;
+  static constexpr int kRawStages = PLANES == 1 ? 4 : 8;
+  // A converter group sees every kWgConvGroups-th k-block.  It must see every
+  // use of a slot that it waits on: were uses skipped, a wait for one phase
+  // parity could not tell the use before the awaited one from the awaited one.
+  static_assert(kBStages % kWgConvGroups == 0 && kRawStages % kWgConvGroups == 0, "a slot belongs to one group");
   static constexpr int kStagingBytes = kWgEpiWarps * 32 * 17 * 4;
-  static constexpr int kFit = (232448 - 1024 - 256 - kStagingBytes) / (kStageBytes + kCodeBytes);
-  static constexpr int kStages = kFit < 8 ? kFit : 8;
-  static constexpr int kBarrierBytes = (3 * kStages + 4) * 8 + 16;
-  static constexpr int kTotal = kStages * (kStageBytes + kCodeBytes) + kBarrierBytes + kStagingBytes + 1024;
+  // One commit a k-block, to a ring of "done" barriers that delta's producer
+  // (kAStages behind) and the converters (kBStages behind) both wait on.
+  static constexpr int kDone = PLANES == 1 ? 12 : 20;
+  static_assert(kDone % kAStages == 0 && kDone % kBStages == 0, "a slot's done barriers repeat with it");
+  static constexpr int kBars = kAStages + kBStages + 2 * kRawStages + kDone + 4;
+  static constexpr int kOffB = kAStages * PLANES * kABytes;
+  static constexpr int kOffRaw = kOffB + kBStages * kBBytes;
+  static constexpr int kOffCodes = kOffRaw + kRawStages * kRawBytes;
+  static constexpr int kOffStaging = kOffCodes + kRawStages * kCodeBytes;
+  static constexpr int kOffBars = kOffStaging + kStagingBytes;
+  static constexpr int kTotal = kOffBars + kBars * 8 + 16 + 1024;
   static constexpr int kChainBlocks = kWgChain / (PLANES * BK / 16);  // k-blocks of one chain
-  static_assert(kTotal <= 232448 && kStages >= 2, "shared memory budget");
+  static_assert(kTotal <= 232448, "shared memory budget");
+};
+
+// Position in a ring of N slots: the slot, and the parity of its use.
+template <int N>
+struct WgRing {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == N) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
 };
 
 // Instruction descriptor with both operands MN-major; F16 or BF16.
@@ -154,52 +199,79 @@ __host__ __device__ constexpr uint32_t wgrad_idesc(bool f16) {
              : umma_idesc_bf16(kWgTileM, kWgTileN, true, true);
 }
 
-__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
-__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ uint32_t add_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
-// 2^e (NaN for code 255) twice in 16-bit halves.  A BF16's exponent field is
-// FP32's.
+// Four int8 values -> four 16-bit x^ = q * 2^e, exactly, as the pairs (0, 2)
+// and (1, 3): what masks give without a byte permutation.  The tile's columns
+// stay in that order and the epilogue swaps the two in the middle of every
+// four back.  The 16-bit float pipe is the converters' limit (32 lanes a clock
+// and SM), so the scale enters through exponent bits and one addition a pair
+// is all it does:
+//   BF16: q's low 7 bits as the mantissa of 128 * 2^e, minus 128 * 2^e or, for
+//         a negative q, 256 * 2^e (the sign bit added to the exponent field)
+//   F16:  q + 128 in the mantissa of 1024 * 2^e, minus 1152 * 2^e
+// That needs these powers of two to be normal numbers of the type.
+// `dequant4_any` works for every code, NaN's included.
 template <bool F16>
-__device__ __forceinline__ uint32_t scale_pair(uint32_t code) {
-  if (F16) {
-    const uint32_t h = __half_as_ushort(__float2half_rn(code_scale(code)));
-    return h | (h << 16);
+struct Dequant {
+  // codes of the short form: e in [-24, 5], or up to 119
+  static constexpr uint32_t kFirst = F16 ? 127 - 24 : 0, kLast = F16 ? 127 + 5 : 127 + 119;
+  uint32_t base, minus;
+  __device__ __forceinline__ static bool fits(uint32_t code) { return code - kFirst <= kLast - kFirst; }
+  __device__ __forceinline__ explicit Dequant(uint32_t code) {
+    if (F16) {
+      const uint32_t h = (code - 127 + 25) << 10;  // 1024 * 2^e
+      base = h | (h << 16);
+      minus = base | 0x80808080u;  // 1152 = 1024 + 128: mantissa bit 7, and the sign (bit 15)
+    } else {
+      const uint32_t h = (code + 7) << 7;  // 128 * 2^e
+      base = h | (h << 16);
+      minus = base | 0x80008000u;
+    }
   }
-  const uint32_t h = code == kCodeNan ? 0x7fffu : code << 7;
-  return h | (h << 16);
-}
+  __device__ __forceinline__ uint2 operator()(uint32_t w) const {
+    if (F16) {
+      const uint32_t u = w ^ 0x80808080u;
+      return make_uint2(add_f16x2((u & 0x00ff00ffu) | base, minus), add_f16x2(((u >> 8) & 0x00ff00ffu) | base, minus));
+    }
+    const uint32_t v = w >> 8;
+    return make_uint2(add_bf16x2((w & 0x007f007fu) | base, (w & 0x00800080u) + minus),
+                      add_bf16x2((v & 0x007f007fu) | base, (v & 0x00800080u) + minus));
+  }
+};
 
-// Four int8 values -> four 16-bit x^ (two words), exactly.
-//   F16:  the byte q + 128 in the mantissa of 1024 gives 1152 + q.
-//   BF16: 7 mantissa bits hold only q's low 7 bits: 128 + (q & 127), from
-//         which 128 or, for a negative q, 256 is taken.  Both constants come
-//         from 0x4300 by setting the sign bit of q as the exponent's lowest bit.
 template <bool F16>
-__device__ __forceinline__ uint2 dequant4(uint32_t w, uint32_t scale) {
+__device__ __noinline__ uint2 dequant4_any(uint32_t w, uint32_t code) {
+  const float scale = code_scale(code);
   if (F16) {
-    const uint32_t u = w ^ 0x80808080u;
-    const uint32_t k = 0x64806480u;  // 1152
-    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-    return make_uint2(mul_f16x2(sub_f16x2(a, k), scale), mul_f16x2(sub_f16x2(b, k), scale));
+    const uint32_t h = __half_as_ushort(__float2half_rn(scale)), s = h | (h << 16);
+    const uint32_t u = w ^ 0x80808080u, m = 0x64006400u, k = 0xe480e480u;  // 1024, -1152
+    return make_uint2(mul_f16x2(add_f16x2((u & 0x00ff00ffu) | m, k), s),
+                      mul_f16x2(add_f16x2(((u >> 8) & 0x00ff00ffu) | m, k), s));
   }
-  const uint32_t a = __byte_perm(w, 0u, 0x4140), b = __byte_perm(w, 0u, 0x4342);
-  const uint32_t m = 0x43004300u;
-  return make_uint2(mul_bf16x2(sub_bf16x2((a & 0x007f007fu) | m, (a & 0x00800080u) | m), scale),
-                    mul_bf16x2(sub_bf16x2((b & 0x007f007fu) | m, (b & 0x00800080u) | m), scale));
+  const uint32_t h = __bfloat16_as_ushort(__float2bfloat16_rn(scale)), s = h | (h << 16);
+  const uint32_t v = w >> 8, m = 0x43004300u, n = 0xc300c300u;  // 128, -128
+  return make_uint2(mul_bf16x2(add_bf16x2((w & 0x007f007fu) | m, (w & 0x00800080u) | n), s),
+                    mul_bf16x2(add_bf16x2((v & 0x007f007fu) | m, (v & 0x00800080u) | n), s));
 }
 
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
@@ -207,8 +279,19 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ uint32_t lds8(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+  return p != 0;
 }
 
 // Arrival on a cluster CTA's barrier in the default (CTA) scope.
@@ -225,15 +308,21 @@ __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+// 32 lanes x 16 consecutive 32-bit columns.
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -289,43 +378,48 @@ __device__ __forceinline__ int64_t partial_offset(int cta, int quarter, int chun
 template <int PLANES, bool F16, int BK, typename OUT>
 __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__ WgradArgs p) {
   using S = WgSmem<PLANES, BK>;
-  constexpr int kStages = S::kStages;
   constexpr uint32_t kChunkBytes = Swz::chunk_bytes(BK);
   constexpr uint32_t kIdesc = wgrad_idesc(F16);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * S::kStageBytes);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * kStages + 4);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kOffBars);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* staging = reinterpret_cast<float*>(smem + kStages * S::kStageBytes + S::kBarrierBytes);
-  uint8_t* code_slots = reinterpret_cast<uint8_t*>(staging) + S::kStagingBytes;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int worker = static_cast<int>(blockIdx.x) / 2;
+  const uint32_t smem_base = smem_u32(smem);
   const uint32_t bar_base = smem_u32(bars);
-  // full: delta bytes of both CTAs + the converters of both (leader's only);
-  // raw: this CTA's int8 tile and its codes; empty: the MMAs that read the slot are done
-  auto bar_full = [&](int s) { return bar_base + 8u * s; };
-  auto bar_raw = [&](int s) { return bar_base + 8u * (kStages + s); };
-  auto bar_empty = [&](int s) { return bar_base + 8u * (2 * kStages + s); };
-  auto bar_tfull = [&](int a) { return bar_base + 8u * (3 * kStages + a); };
-  auto bar_tempty = [&](int a) { return bar_base + 8u * (3 * kStages + 2 + a); };
-  auto slot_a = [&](int s) { return smem_u32(smem + s * S::kStageBytes); };
-  auto slot_b = [&](int s) { return smem_u32(smem + s * S::kStageBytes + PLANES * S::kABytes); };
-  auto slot_raw = [&](int s) { return smem_u32(smem + s * S::kStageBytes + PLANES * S::kABytes + S::kBBytes); };
+  // a_full (the leader's): delta bytes of both CTAs.  b_full (the leader's): the
+  // converters of both CTAs.  done: the MMAs of a k-block are done, in both
+  // CTAs.  raw_full: this CTA's int8 tile and its codes.  raw_empty: its
+  // converters have read it.
+  auto bar_afull = [&](int i) { return bar_base + 8u * i; };
+  auto bar_bfull = [&](int i) { return bar_base + 8u * (S::kAStages + i); };
+  auto bar_done = [&](int i) { return bar_base + 8u * (S::kAStages + S::kBStages + i); };
+  auto bar_rfull = [&](int i) { return bar_base + 8u * (S::kAStages + S::kBStages + S::kDone + i); };
+  auto bar_rempty = [&](int i) { return bar_base + 8u * (S::kAStages + S::kBStages + S::kDone + S::kRawStages + i); };
+  auto bar_tfull = [&](int i) { return bar_base + 8u * (S::kBars - 4 + i); };
+  auto bar_tempty = [&](int i) { return bar_base + 8u * (S::kBars - 2 + i); };
+  auto slot_a = [&](int i) { return smem_base + i * (PLANES * S::kABytes); };
+  auto slot_b = [&](int i) { return smem_base + S::kOffB + i * S::kBBytes; };
+  auto slot_raw = [&](int i) { return smem_base + S::kOffRaw + i * S::kRawBytes; };
+  auto slot_codes = [&](int i) { return smem_base + S::kOffCodes + i * S::kCodeBytes; };
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(bar_full(s), 1 + 2 * kWgConvWarps);
-      mbar_init(bar_raw(s), 1 + 32);
-      mbar_init(bar_empty(s), 1);
+    for (int i = 0; i < S::kAStages; ++i) mbar_init(bar_afull(i), 1);
+    for (int i = 0; i < S::kBStages; ++i) mbar_init(bar_bfull(i), 2 * kWgConvWarps / kWgConvGroups);
+    for (int i = 0; i < S::kDone; ++i) mbar_init(bar_done(i), 1);
+    for (int i = 0; i < S::kRawStages; ++i) {
+      mbar_init(bar_rfull(i), 1 + 32);
+      mbar_init(bar_rempty(i), kWgConvWarps / kWgConvGroups);
     }
-    for (int a = 0; a < 2; ++a) {
-      mbar_init(bar_tfull(a), 1);
-      mbar_init(bar_tempty(a), 2 * kWgEpiWarps);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar_tfull(i), 1);
+      mbar_init(bar_tempty(i), 2 * kWgEpiWarps);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -350,121 +444,150 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
   grid_dep_launch();
 
   if (warp == 0) {
-    // ------------------------------------------------------------ producer
-    int stage = 0;
-    uint32_t phase = 0;
+    // ------------------------------------------------------ delta producer
+    if (lane == 0) {
+      WgRing<S::kAStages> ra;
+      WgRing<S::kDone> rd;  // the k-block kAStages back
+      int64_t i = 0;
+      bool ok = true;
+      for (WgIter it(p, worker); it.valid() && ok;) {
+        const WgSegment s = it.get();
+        const int mc = s.mi * kWgTileM + static_cast<int>(rank) * 128;
+        for (int kb = s.kb0; kb < s.kb1; ++kb, ++i, ra.next()) {
+          if (i >= S::kAStages) {
+            if (!mbar_wait(bar_done(rd.slot), rd.phase, abort_flag, kStatusTimeoutWgradProducer)) {
+              ok = false;
+              break;
+            }
+            rd.next();
+          }
+          const uint32_t fb = mapa_shared(bar_afull(ra.slot), 0);
+          if (rank == 0) mbar_arrive_expect_tx(bar_afull(ra.slot), 2 * PLANES * S::kABytes);
+#pragma unroll
+          for (int j = 0; j < PLANES; ++j) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              tma_load_2d_pair(slot_a(ra.slot) + j * S::kABytes + h * kChunkBytes, &p.a[j], fb, mc + 64 * h, kb * BK);
+          }
+        }
+        it.next(s);
+      }
+      // the leader's last commits have arrived before this CTA may leave
+      for (int64_t left = i < S::kAStages ? i : S::kAStages; left > 0 && ok; --left, rd.next())
+        ok = mbar_wait(bar_done(rd.slot), rd.phase, abort_flag, kStatusTimeoutWgradProducer);
+    }
+  } else if (warp == kWgRawWarp) {
+    // -------------------------------------------------------- raw producer
+    // (apart from delta's, whose waits for the MMAs would hold it back)
+    WgRing<S::kRawStages> rr;
     bool ok = true;
     for (WgIter it(p, worker); it.valid() && ok;) {
       const WgSegment s = it.get();
-      const int mc = s.tile / p.tiles_n * kWgTileM + static_cast<int>(rank) * 128;
-      const int nc = s.tile % p.tiles_n * kWgTileN + static_cast<int>(rank) * 128;
+      const int nc = s.ni * kWgTileN + static_cast<int>(rank) * 128;
       const bool c_ok = nc / kGroup < p.lde;
       for (int kb = s.kb0; kb < s.kb1; ++kb) {
-        ok = mbar_wait(bar_empty(stage), phase ^ 1u, abort_flag, kStatusTimeoutWgradProducer);
+        ok = mbar_wait(bar_rempty(rr.slot), rr.phase ^ 1u, abort_flag, kStatusTimeoutWgradProducer);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
         }
         if (lane == 0) {
-          mbar_arrive_expect_tx(bar_raw(stage), S::kRawBytes);
-          tma_load_2d(slot_raw(stage), &p.q, bar_raw(stage), nc, kb * BK);
-          const uint32_t fb = mapa_shared(bar_full(stage), 0);
-          if (rank == 0) mbar_arrive_expect_tx(bar_full(stage), 2 * PLANES * S::kABytes);
-#pragma unroll
-          for (int j = 0; j < PLANES; ++j) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              tma_load_2d_pair(slot_a(stage) + j * S::kABytes + h * kChunkBytes, &p.a[j], fb, mc + 64 * h, kb * BK);
-          }
+          mbar_arrive_expect_tx(bar_rfull(rr.slot), S::kRawBytes);
+          tma_load_2d(slot_raw(rr.slot), &p.q, bar_rfull(rr.slot), nc, kb * BK);
         }
         // codes outside the checkpoint become 0: their values are 0 as well
 #pragma unroll
         for (int t = 0; t < BK / 32; ++t) {
           const int k = t * 32 + lane, r = kb * BK + k;
           const bool r_ok = c_ok && r < p.rows;
-          cp_async4(smem_u32(code_slots + stage * S::kCodeBytes) + 4 * k,
+          cp_async4(slot_codes(rr.slot) + 4 * k,
                     p.codes + (r_ok ? static_cast<int64_t>(r) * p.lde + nc / kGroup : 0), r_ok);
         }
-        cp_async_arrive(bar_raw(stage));
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
+        cp_async_arrive(bar_rfull(rr.slot));
+        rr.next();
       }
       it.next(s);
     }
-    // every slot's last release (a commit of the leader) has arrived before
-    // this CTA may leave
-    for (int i = 0; i < kStages && ok; ++i) {
-      ok = mbar_wait(bar_empty(stage), phase ^ 1u, abort_flag, kStatusTimeoutWgradProducer);
-      if (++stage == kStages) {
-        stage = 0;
-        phase ^= 1u;
-      }
-    }
+    // the converters have read every slot
+    for (int i = 0; i < S::kRawStages && ok; ++i, rr.next())
+      ok = mbar_wait(bar_rempty(rr.slot), rr.phase ^ 1u, abort_flag, kStatusTimeoutWgradProducer);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
-    if (lane == 0 && rank == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
+    // The whole warp walks the loop, so that descriptors and barriers stay in
+    // uniform registers; one elected lane issues.  (One lane alone in a
+    // divergent branch took 95 clocks an MMA, longer than its 128 allow for.)
+    if (rank == 0) {
+      const bool elected = elect_one();
+      WgRing<S::kAStages> ra;
+      WgRing<S::kBStages> rb;
+      WgRing<S::kDone> rd;
       int home = 0;
       uint32_t uses0 = 0, uses1 = 0;  // chains that ran in each accumulator
       bool ok = true;
+      const uint64_t a_desc = umma_desc(slot_a(0), kChunkBytes, Swz::kSbo, Swz::kLayout);
+      const uint64_t b_desc = umma_desc(slot_b(0), kChunkBytes, Swz::kSbo, Swz::kLayout);
       for (WgIter it(p, worker); it.valid() && ok; home ^= 1) {
         const WgSegment s = it.get();
         for (int begin = s.kb0; begin < s.kb1 && ok; begin += S::kChainBlocks) {
           const int end = min(begin + S::kChainBlocks, s.kb1);
           const int acc = begin == s.kb0 ? home : home ^ 1;
           const uint32_t uses = acc ? uses1++ : uses0++;
-          if (!mbar_wait(bar_tempty(acc), (uses & 1) ^ 1u, abort_flag, kStatusTimeoutWgradMma)) {
+          ok = mbar_wait(bar_tempty(acc), (uses & 1) ^ 1u, abort_flag, kStatusTimeoutWgradMma);
+          if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
           }
           tc_fence_after();
           const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kWgTileN);
           for (int kb = begin; kb < end; ++kb) {
-            if (!mbar_wait(bar_full(stage), phase, abort_flag, kStatusTimeoutWgradMma)) {
+            ok = mbar_wait(bar_afull(ra.slot), ra.phase, abort_flag, kStatusTimeoutWgradMma) &&
+                 mbar_wait(bar_bfull(rb.slot), rb.phase, abort_flag, kStatusTimeoutWgradMma);
+            if (!__all_sync(0xffffffffu, ok)) {
               ok = false;
               break;
             }
             tc_fence_after();
+            // the start address is in units of 16 bytes in the lowest bits
+            const uint64_t a0 = a_desc + static_cast<uint32_t>(ra.slot) * (PLANES * S::kABytes / 16);
+            const uint64_t b0 = b_desc + static_cast<uint32_t>(rb.slot) * (S::kBBytes / 16);
+            if (elected) {
 #pragma unroll
-            for (int ks = 0; ks < BK / 16; ++ks) {
-              const uint64_t b =
-                  umma_desc(slot_b(stage) + ks * Swz::kMnStepBytes, kChunkBytes, Swz::kSbo, Swz::kLayout);
+              for (int ks = 0; ks < BK / 16; ++ks) {
 #pragma unroll
-              for (int j = PLANES - 1; j >= 0; --j) {  // smallest plane first
-                const uint64_t a = umma_desc(slot_a(stage) + j * S::kABytes + ks * Swz::kMnStepBytes, kChunkBytes,
-                                             Swz::kSbo, Swz::kLayout);
-                umma_bf16_pair(d_tmem, a, b, kIdesc, (kb > begin || ks > 0 || j < PLANES - 1) ? 1u : 0u);
+                for (int j = PLANES - 1; j >= 0; --j)  // smallest plane first
+                  umma_bf16_pair(d_tmem, a0 + (j * S::kABytes + ks * Swz::kMnStepBytes) / 16,
+                                 b0 + ks * Swz::kMnStepBytes / 16, kIdesc,
+                                 (kb > begin || ks > 0 || j < PLANES - 1) ? 1u : 0u);
               }
+              umma_commit_pair(bar_done(rd.slot), 0x3);
             }
-            umma_commit_pair(bar_empty(stage), 0x3);
-            if (++stage == kStages) {
-              stage = 0;
-              phase ^= 1u;
-            }
+            __syncwarp();
+            ra.next();
+            rb.next();
+            rd.next();
           }
-          if (ok) umma_commit_pair(bar_tfull(acc), 0x3);
+          if (ok && elected) umma_commit_pair(bar_tfull(acc), 0x3);
+          __syncwarp();
         }
         it.next(s);
       }
       // both accumulators' last chains have been read by both CTAs
       if (ok) ok = mbar_wait(bar_tempty(0), (uses0 & 1) ^ 1u, abort_flag, kStatusTimeoutWgradMma);
       if (ok) mbar_wait(bar_tempty(1), (uses1 & 1) ^ 1u, abort_flag, kStatusTimeoutWgradMma);
+      __syncwarp();
     }
   } else if (warp < 2 + kWgEpiWarps) {
     // ------------------------------------------------------------ epilogue
     const int quarter = warp & 3;           // TMEM lanes this warp may access
     const int half = (warp - 2) >> 2;       // its 128 of the tile's 256 columns
     const uint32_t tempty0 = mapa_shared(bar_tempty(0), 0);
-    float* stg = staging + (warp - 2) * 32 * 17;
+    float* stg = reinterpret_cast<float*>(smem + S::kOffStaging) + (warp - 2) * 32 * 17;
     auto release = [&](int acc) {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(tempty0 + 8u * acc);
+      if (lane == 0) mbar_arrive_remote(tempty0 + 8u * acc);
     };
     int home = 0;
     uint32_t uses0 = 0, uses1 = 0;
@@ -472,8 +595,8 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
     for (WgIter it(p, worker); it.valid() && ok; home ^= 1) {
       const WgSegment s = it.get();
       const bool whole = s.kb0 == 0 && s.kb1 == p.kblocks;
-      const int row0 = s.tile / p.tiles_n * kWgTileM + static_cast<int>(rank) * 128 + quarter * 32;
-      const int colt = s.tile % p.tiles_n * kWgTileN;
+      const int row0 = s.mi * kWgTileM + static_cast<int>(rank) * 128 + quarter * 32;
+      const int colt = s.ni * kWgTileN;
       float* part = p.partials + static_cast<int64_t>(2 * worker + (it.index > 0 ? 1 : 0)) * kWgPartialFloats;
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
       const uint32_t t_home = t_row + static_cast<uint32_t>(home * kWgTileN);
@@ -490,40 +613,45 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
         }
         tc_fence_after();
         if (first && !last) continue;  // stays in the home accumulator
+        constexpr int kSteps = kWgTileN / 2 / 16;  // 16 columns each
 #pragma unroll 1
-        for (int j = 4 * half; j < 4 * half + 4; ++j) {
-          uint32_t r[32];
-          tmem_ld_32x32(t_home + j * 32, r);
+        for (int i = 0; i < kSteps; ++i) {
+          const int col = kWgTileN / 2 * half + 16 * i;
+          uint32_t r[16];
+          tmem_ld_32x16(t_home + col, r);
           if (!first) {
-            uint32_t x[32];
-            tmem_ld_32x32(t_other + j * 32, x);
+            uint32_t x[16];
+            tmem_ld_32x16(t_other + col, x);
             tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) + __uint_as_float(x[c]));
-            if (j == 4 * half + 3) release(home ^ 1);
+            for (int c = 0; c < 16; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) + __uint_as_float(x[c]));
+            if (i == kSteps - 1) release(home ^ 1);
           } else {
             tmem_wait_ld();
           }
           if (!last) {
-            tmem_st_32x32(t_home + j * 32, r);
+            tmem_st_32x16(t_home + col, r);
             continue;
           }
-          if (j == 4 * half + 3) release(home);
+          if (i == kSteps - 1) release(home);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {  // the converters' column order back to the result's
+            const uint32_t swap = r[4 * c + 1];
+            r[4 * c + 1] = r[4 * c + 2];
+            r[4 * c + 2] = swap;
+          }
           if (!whole) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-              *reinterpret_cast<uint4*>(part + partial_offset(rank, quarter, j, c, lane)) =
+            for (int c = 0; c < 4; ++c)
+              *reinterpret_cast<uint4*>(part + partial_offset(rank, quarter, col / 32, col / 4 % 8 + c, lane)) =
                   make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
           } else {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-              for (int c = 0; c < 16; ++c) stg[lane * 17 + c] = __uint_as_float(r[16 * h + c]);
-              __syncwarp();
-              store_block<16>(static_cast<OUT*>(p.out), p.d_in, row0, colt + 32 * j + 16 * h, p.d_out, p.d_in, stg,
-                              lane, p.vec_out != 0);
-              __syncwarp();
-            }
+            for (int c = 0; c < 16; ++c) stg[lane * 17 + c] = __uint_as_float(r[c]);
+            __syncwarp();
+            store_block<16>(static_cast<OUT*>(p.out), p.d_in, row0, colt + col, p.d_out, p.d_in, stg, lane,
+                            p.vec_out != 0);
+            __syncwarp();
           }
         }
         if (!last) tmem_wait_st();
@@ -532,49 +660,59 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
     }
   } else {
     // ---------------------------------------------------------- converters
-    // A task is 16 columns of one token: 8 lanes cover a token's 128 columns.
-    constexpr int kTasks = BK * 8 / (32 * kWgConvWarps);
-    static_assert(kTasks * 32 * kWgConvWarps == BK * 8, "whole tasks per thread");
-    const int tid = threadIdx.x - 32 * (2 + kWgEpiWarps);
-    const int seg = tid & 7, k0 = tid >> 3;  // k0 < 32; a thread's tokens are 32 apart
-    const uint32_t full0 = mapa_shared(bar_base, 0);
-    // Offsets inside a slot.  Tokens 32 apart have the same swizzle; lanes of
-    // the two 64-column chunks store their halves in opposite order, so that
-    // no bank is hit twice.
-    const bool flip = (seg & 4) != 0;
-    const uint32_t u = (seg & 3) * 2;
-    const uint32_t in_off = k0 * 128 + seg * 16;
-    const uint32_t row_off = (seg >> 2) * kChunkBytes + k0 * 128;
-    const uint32_t off0 = row_off + (((u + flip) ^ (k0 & 7)) << 4);
-    const uint32_t off1 = row_off + (((u + !flip) ^ (k0 & 7)) << 4);
-    const uint32_t code_off = 4 * k0 + (seg >> 1);
-    int stage = 0;
-    uint32_t phase = 0;
-    int64_t left = 0;
-    for (WgIter it(p, worker); it.valid();) {
-      const WgSegment s = it.get();
-      left += s.kb1 - s.kb0;
-      it.next(s);
-    }
-    for (; left > 0; --left) {
-      const bool ok = mbar_wait(bar_raw(stage), phase, abort_flag, kStatusTimeoutWgradConvert);
+    // Groups of warps take k-blocks in turn, so that one group's latency hides
+    // behind the other's.  A task is 16 columns of one token.  8 neighbouring
+    // lanes hold 4 tasks of token k in one 64-column chunk and 4 of token k ^ 1
+    // in the other: their 16-byte loads and swizzled stores each cover all 32
+    // banks once.
+    constexpr int kGroupWarps = kWgConvWarps / kWgConvGroups;
+    constexpr int kTasks = BK * 8 / (32 * kGroupWarps);
+    constexpr int kTaskRows = 4 * kGroupWarps;  // tokens of one task round, a multiple of the swizzle's 8
+    static_assert(kTaskRows % 8 == 0 && kTasks * kTaskRows == BK, "whole task rounds");
+    const int group = (warp - 2 - kWgEpiWarps) / kGroupWarps;
+    const int k0 = ((warp - 2 - kWgEpiWarps) % kGroupWarps) * 4 + (lane >> 4) * 2 + ((lane >> 2) & 1);
+    const int chunk = ((lane >> 3) ^ k0) & 1, seg = lane & 3;
+    const uint32_t in_off = k0 * 128 + chunk * 64 + seg * 16;
+    const uint32_t out_off = chunk * kChunkBytes + k0 * 128;
+    const uint32_t off0 = out_off + (((2 * seg) ^ (k0 & 7)) << 4), off1 = out_off + (((2 * seg + 1) ^ (k0 & 7)) << 4);
+    const uint32_t code_off = 4 * k0 + 2 * chunk + (seg >> 1);
+    const uint32_t bfull0 = mapa_shared(bar_bfull(0), 0);
+    WgRing<S::kRawStages> rr;
+    WgRing<S::kBStages> rb;
+    WgRing<S::kDone> rd;  // the k-block kBStages back
+    // k-blocks of this worker: its share and its whole tiles
+    const int64_t whole = p.shared + worker < p.tiles ? (p.tiles - 1 - p.shared - worker) / p.workers + 1 : 0;
+    const int64_t blocks = wgrad_begin(p, worker + 1) - wgrad_begin(p, worker) + whole * p.kblocks;
+    for (int64_t i = 0; i < blocks; ++i, rr.next(), rb.next()) {
+      if (i > S::kBStages) rd.next();
+      if (kWgConvGroups > 1 && i % kWgConvGroups != group) continue;
+      bool ok = mbar_wait(bar_rfull(rr.slot), rr.phase, abort_flag, kStatusTimeoutWgradConvert);
       if (!__all_sync(0xffffffffu, ok)) break;
-      const uint32_t raw = slot_raw(stage) + in_off, out = slot_b(stage);
-      const uint8_t* codes = code_slots + stage * S::kCodeBytes + code_off;
       uint4 w[kTasks];
       uint32_t code[kTasks];
 #pragma unroll
       for (int t = 0; t < kTasks; ++t) {
-        w[t] = lds128(raw + t * 32 * 128);
-        code[t] = codes[t * 128];
+        w[t] = lds128(slot_raw(rr.slot) + in_off + t * (kTaskRows * 128));
+        code[t] = lds8(slot_codes(rr.slot) + code_off + t * (kTaskRows * 4));
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_rempty(rr.slot));
+      if (i >= S::kBStages) {
+        ok = mbar_wait(bar_done(rd.slot), rd.phase, abort_flag, kStatusTimeoutWgradConvert);
+        if (!__all_sync(0xffffffffu, ok)) break;
       }
 #pragma unroll
       for (int t = 0; t < kTasks; ++t) {
-        const uint32_t sc = scale_pair<F16>(code[t]);
-        const uint2 a0 = dequant4<F16>(flip ? w[t].z : w[t].x, sc), a1 = dequant4<F16>(flip ? w[t].w : w[t].y, sc);
-        const uint2 b0 = dequant4<F16>(flip ? w[t].x : w[t].z, sc), b1 = dequant4<F16>(flip ? w[t].y : w[t].w, sc);
-        sts128(out + off0 + t * 32 * 128, a0.x, a0.y, a1.x, a1.y);
-        sts128(out + off1 + t * 32 * 128, b0.x, b0.y, b1.x, b1.y);
+        uint2 a0, a1, b0, b1;
+        if (Dequant<F16>::fits(code[t])) {
+          const Dequant<F16> d(code[t]);
+          a0 = d(w[t].x), a1 = d(w[t].y), b0 = d(w[t].z), b1 = d(w[t].w);
+        } else {
+          a0 = dequant4_any<F16>(w[t].x, code[t]), a1 = dequant4_any<F16>(w[t].y, code[t]);
+          b0 = dequant4_any<F16>(w[t].z, code[t]), b1 = dequant4_any<F16>(w[t].w, code[t]);
+        }
+        sts128(slot_b(rb.slot) + off0 + t * (kTaskRows * 128), a0.x, a0.y, a1.x, a1.y);
+        sts128(slot_b(rb.slot) + off1 + t * (kTaskRows * 128), b0.x, b0.y, b1.x, b1.y);
       }
       // The MMA that these arrivals admit reads this tile through this CTA's
       // own async proxy, to which the fence has made it visible; no data is
@@ -583,11 +721,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
       // of 614 for 16384 x 2048 x 8192).
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive_remote(full0 + 8u * stage);
-      if (++stage == kStages) {
-        stage = 0;
-        phase ^= 1u;
-      }
+      if (lane == 0) mbar_arrive_remote(bfull0 + 8u * rb.slot);
     }
   }
 
@@ -611,18 +745,11 @@ __global__ void __launch_bounds__(256) k_wgrad_join(const __grid_constant__ Wgra
   const int tile = blockIdx.x;
   const int block = blockIdx.y;  // [cta][quarter][chunk]
   const int cta = block >> 5, quarter = (block >> 3) & 3, chunk = block & 7;
-  const int row0 = tile / p.tiles_n * kWgTileM + cta * 128 + quarter * 32;
-  const int col0 = tile % p.tiles_n * kWgTileN + chunk * 32;
-  const int64_t k_begin = static_cast<int64_t>(tile) * p.kblocks;
-  // the worker that holds k-block b: the largest w with begin(w) <= b
-  auto worker_of = [&](int64_t b) {
-    int w = p.parts > 0 ? static_cast<int>(b / p.kblocks * p.parts + b % p.kblocks * p.parts / p.kblocks)
-                        : static_cast<int>(b * p.workers / (static_cast<int64_t>(p.shared) * p.kblocks));
-    while (w + 1 < p.workers && wgrad_begin(p, w + 1) <= b) ++w;
-    while (w > 0 && wgrad_begin(p, w) > b) --w;
-    return w;
-  };
-  const int w0 = worker_of(k_begin), w1 = worker_of(k_begin + p.kblocks - 1);
+  const int mi = tile / p.tiles_n;
+  const int row0 = mi * kWgTileM + cta * 128 + quarter * 32;
+  const int col0 = (tile - mi * p.tiles_n) * kWgTileN + chunk * 32;
+  const int k_begin = tile * p.kblocks;
+  const int w0 = wgrad_worker(p, k_begin), w1 = wgrad_worker(p, k_begin + p.kblocks - 1);
   // a worker's first segment is in its slot 0, a later one (its last) in slot 1
   const bool late = wgrad_begin(p, w0) < k_begin;
   grid_dep_wait();
