@@ -15,11 +15,11 @@
 //   warp 0        delta producer: TMA loads (128-byte swizzle), counted on the
 //                 leader's barrier
 //   warp 1        MMA issuer (the leader's thread, for both CTAs)
-//   warps 2..9    epilogue: TMEM -> registers -> global
-//   warps 10..25  converters: raw int8 tile -> 16-bit x^ in the swizzled layout
+//   warp 2        raw producer: TMA loads of the int8 tiles
+//   warp 3        code producer: 4-byte asynchronous copies of their exponents
+//   warps 4..11   epilogue: TMEM -> registers -> global
+//   warps 12..27  converters: raw int8 tile -> 16-bit x^ in the swizzled layout
 //                 the MMA reads, then an arrival on the leader's barrier
-//   warp 26       raw producer: TMA loads of the int8 tiles and 4-byte
-//                 asynchronous copies of their exponent codes
 //
 // The tensor core's FP32 accumulation truncates, so its error grows with the
 // length of a chain of MMAs (7e-6 relative after 1024 steps of 16 tokens).  A
@@ -50,8 +50,15 @@ constexpr int kWgConvWarps = 16;
 constexpr int kWgConvGroups = 4;
 constexpr int kWgEpiWarps = 8;
 constexpr int kWgChain = 128;  // MMA steps summed by the tensor core alone
-constexpr int kWgRawWarp = 2 + kWgEpiWarps + kWgConvWarps;
-constexpr int kWgThreads = 32 * (kWgRawWarp + 1);
+// Warps 0..3 issue loads and MMAs; then come the epilogue and the converters, each whole groups of four warps that trade registers
+// (setmaxnreg): the launch's 28 warps of 72 cover 4 of 40, 8 of 104 and 16 of 64.
+constexpr int kWgEpiWarp0 = 4, kWgConvWarp0 = kWgEpiWarp0 + kWgEpiWarps;
+constexpr int kWgThreads = 32 * (kWgConvWarp0 + kWgConvWarps);
+constexpr int kWgLaunchRegs = 72, kWgIssueRegs = 40, kWgEpiRegs = 104, kWgConvRegs = 64;
+static_assert(kWgThreads * kWgLaunchRegs <= 65536 &&
+                  32 * (kWgEpiWarp0 * kWgIssueRegs + kWgEpiWarps * kWgEpiRegs + kWgConvWarps * kWgConvRegs) <=
+                      kWgThreads * kWgLaunchRegs,
+              "the register split fits what the block is launched with");
 constexpr int kWgPartialFloats = kWgTileM * kWgTileN;
 // k-blocks of one worker's share are at least this many (256 tokens), so that
 // a short sum is not cut into partial tiles that cost more than they save
@@ -157,19 +164,21 @@ struct WgSmem {
   static constexpr int kBBytes = 128 * BK * 2;    // this CTA's x^ columns
   static constexpr int kRawBytes = 128 * BK;
   static constexpr int kCodeBytes = 4 * BK;       // exponent codes of a raw tile
-  static constexpr int kAStages = PLANES == 1 ? 6 : 5;
+  static constexpr int kAStages = 5;
   static constexpr int kBStages = 4;
-  static constexpr int kRawStages = PLANES == 1 ? 4 : 8;
+  static constexpr int kRawStages = 8;
   // A converter group sees every kWgConvGroups-th k-block.  It must see every
   // use of a slot that it waits on: were uses skipped, a wait for one phase
   // parity could not tell the use before the awaited one from the awaited one.
-  static_assert(kBStages % kWgConvGroups == 0 && kRawStages % kWgConvGroups == 0, "a slot belongs to one group");
-  static constexpr int kStagingBytes = kWgEpiWarps * 32 * 17 * 4;
-  // One commit a k-block, to a ring of "done" barriers that delta's producer
-  // (kAStages behind) and the converters (kBStages behind) both wait on.
-  static constexpr int kDone = PLANES == 1 ? 12 : 20;
-  static_assert(kDone % kAStages == 0 && kDone % kBStages == 0, "a slot's done barriers repeat with it");
-  static constexpr int kBars = kAStages + kBStages + 2 * kRawStages + kDone + 4;
+  static_assert(kRawStages % kWgConvGroups == 0, "a raw slot belongs to one group");
+  static constexpr int kStagingBytes = kWgEpiWarps * 32 * 9 * 4;
+  // Barriers per k-block, not per slot: "full" (both operands are there) and
+  // "done" (its MMAs are), in rings whose length both slot rings divide.  One
+  // wait and one commit a k-block are what the issuing warp has time for.
+  static constexpr int kRing = 20;
+  static_assert(kRing % kAStages == 0 && kRing % kBStages == 0, "a slot's barriers repeat with it");
+  static_assert(kRing % kWgConvGroups == 0, "a done barrier belongs to one group");
+  static constexpr int kBars = 2 * kRing + 2 * kRawStages + 4;
   static constexpr int kOffB = kAStages * PLANES * kABytes;
   static constexpr int kOffRaw = kOffB + kBStages * kBBytes;
   static constexpr int kOffCodes = kOffRaw + kRawStages * kRawBytes;
@@ -185,9 +194,13 @@ template <int N>
 struct WgRing {
   int slot = 0;
   uint32_t phase = 0;
-  __device__ __forceinline__ void next() {
-    if (++slot == N) {
-      slot = 0;
+  __device__ __forceinline__ void next() { skip<1>(); }
+  // by n uses, where n <= N
+  template <int n>
+  __device__ __forceinline__ void skip() {
+    slot += n;
+    if (slot >= N) {
+      slot -= N;
       phase ^= 1u;
     }
   }
@@ -294,6 +307,20 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+// Whether the phase is complete, without waiting (try_wait may suspend the
+// thread for a while).
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // Arrival on a cluster CTA's barrier in the default (CTA) scope.
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
@@ -317,12 +344,15 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -393,15 +423,13 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
   const int worker = static_cast<int>(blockIdx.x) / 2;
   const uint32_t smem_base = smem_u32(smem);
   const uint32_t bar_base = smem_u32(bars);
-  // a_full (the leader's): delta bytes of both CTAs.  b_full (the leader's): the
-  // converters of both CTAs.  done: the MMAs of a k-block are done, in both
-  // CTAs.  raw_full: this CTA's int8 tile and its codes.  raw_empty: its
-  // converters have read it.
-  auto bar_afull = [&](int i) { return bar_base + 8u * i; };
-  auto bar_bfull = [&](int i) { return bar_base + 8u * (S::kAStages + i); };
-  auto bar_done = [&](int i) { return bar_base + 8u * (S::kAStages + S::kBStages + i); };
-  auto bar_rfull = [&](int i) { return bar_base + 8u * (S::kAStages + S::kBStages + S::kDone + i); };
-  auto bar_rempty = [&](int i) { return bar_base + 8u * (S::kAStages + S::kBStages + S::kDone + S::kRawStages + i); };
+  // full (the leader's): delta bytes and converters of both CTAs.  done: the
+  // MMAs of a k-block are done, in both CTAs.  raw_full: this CTA's int8 tile
+  // and its codes.  raw_empty: its converters have read it.
+  auto bar_full = [&](int i) { return bar_base + 8u * i; };
+  auto bar_done = [&](int i) { return bar_base + 8u * (S::kRing + i); };
+  auto bar_rfull = [&](int i) { return bar_base + 8u * (2 * S::kRing + i); };
+  auto bar_rempty = [&](int i) { return bar_base + 8u * (2 * S::kRing + S::kRawStages + i); };
   auto bar_tfull = [&](int i) { return bar_base + 8u * (S::kBars - 4 + i); };
   auto bar_tempty = [&](int i) { return bar_base + 8u * (S::kBars - 2 + i); };
   auto slot_a = [&](int i) { return smem_base + i * (PLANES * S::kABytes); };
@@ -410,9 +438,10 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
   auto slot_codes = [&](int i) { return smem_base + S::kOffCodes + i * S::kCodeBytes; };
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < S::kAStages; ++i) mbar_init(bar_afull(i), 1);
-    for (int i = 0; i < S::kBStages; ++i) mbar_init(bar_bfull(i), 2 * kWgConvWarps / kWgConvGroups);
-    for (int i = 0; i < S::kDone; ++i) mbar_init(bar_done(i), 1);
+    for (int i = 0; i < S::kRing; ++i) {
+      mbar_init(bar_full(i), 1 + 2 * kWgConvWarps / kWgConvGroups);
+      mbar_init(bar_done(i), 1);
+    }
     for (int i = 0; i < S::kRawStages; ++i) {
       mbar_init(bar_rfull(i), 1 + 32);
       mbar_init(bar_rempty(i), kWgConvWarps / kWgConvGroups);
@@ -443,17 +472,18 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
   grid_dep_wait();
   grid_dep_launch();
 
+  if (warp < kWgEpiWarp0) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWgIssueRegs));
   if (warp == 0) {
     // ------------------------------------------------------ delta producer
     if (lane == 0) {
       WgRing<S::kAStages> ra;
-      WgRing<S::kDone> rd;  // the k-block kAStages back
+      WgRing<S::kRing> rf, rd;  // this k-block, and the one kAStages back
       int64_t i = 0;
       bool ok = true;
       for (WgIter it(p, worker); it.valid() && ok;) {
         const WgSegment s = it.get();
         const int mc = s.mi * kWgTileM + static_cast<int>(rank) * 128;
-        for (int kb = s.kb0; kb < s.kb1; ++kb, ++i, ra.next()) {
+        for (int kb = s.kb0; kb < s.kb1; ++kb, ++i, ra.next(), rf.next()) {
           if (i >= S::kAStages) {
             if (!mbar_wait(bar_done(rd.slot), rd.phase, abort_flag, kStatusTimeoutWgradProducer)) {
               ok = false;
@@ -461,8 +491,8 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
             }
             rd.next();
           }
-          const uint32_t fb = mapa_shared(bar_afull(ra.slot), 0);
-          if (rank == 0) mbar_arrive_expect_tx(bar_afull(ra.slot), 2 * PLANES * S::kABytes);
+          const uint32_t fb = mapa_shared(bar_full(rf.slot), 0);
+          if (rank == 0) mbar_arrive_expect_tx(bar_full(rf.slot), 2 * PLANES * S::kABytes);
 #pragma unroll
           for (int j = 0; j < PLANES; ++j) {
 #pragma unroll
@@ -476,41 +506,54 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
       for (int64_t left = i < S::kAStages ? i : S::kAStages; left > 0 && ok; --left, rd.next())
         ok = mbar_wait(bar_done(rd.slot), rd.phase, abort_flag, kStatusTimeoutWgradProducer);
     }
-  } else if (warp == kWgRawWarp) {
+  } else if (warp == 2) {
     // -------------------------------------------------------- raw producer
     // (apart from delta's, whose waits for the MMAs would hold it back)
+    if (lane == 0) {
+      WgRing<S::kRawStages> rr;
+      bool ok = true;
+      for (WgIter it(p, worker); it.valid() && ok;) {
+        const WgSegment s = it.get();
+        const int nc = s.ni * kWgTileN + static_cast<int>(rank) * 128;
+        for (int kb = s.kb0; kb < s.kb1; ++kb, rr.next()) {
+          if (!mbar_wait(bar_rempty(rr.slot), rr.phase ^ 1u, abort_flag, kStatusTimeoutWgradProducer)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(bar_rfull(rr.slot), S::kRawBytes);
+          tma_load_2d(slot_raw(rr.slot), &p.q, bar_rfull(rr.slot), nc, kb * BK);
+        }
+        it.next(s);
+      }
+      // the converters have read every slot
+      for (int i = 0; i < S::kRawStages && ok; ++i, rr.next())
+        ok = mbar_wait(bar_rempty(rr.slot), rr.phase ^ 1u, abort_flag, kStatusTimeoutWgradProducer);
+    }
+  } else if (warp == 3) {
+    // ------------------------------------------------------- code producer
+    // A lane copies the 4 codes of a token's 128 columns.  Codes outside the
+    // checkpoint become 0: their values are 0 as well.
     WgRing<S::kRawStages> rr;
     bool ok = true;
     for (WgIter it(p, worker); it.valid() && ok;) {
       const WgSegment s = it.get();
-      const int nc = s.ni * kWgTileN + static_cast<int>(rank) * 128;
-      const bool c_ok = nc / kGroup < p.lde;
-      for (int kb = s.kb0; kb < s.kb1; ++kb) {
+      const int g = (s.ni * kWgTileN + static_cast<int>(rank) * 128) / kGroup;
+      const int rows = g < p.lde ? p.rows : 0;
+      const uint8_t* src = p.codes + (static_cast<int64_t>(s.kb0) * BK + lane) * p.lde + g;
+      int r = s.kb0 * BK + lane;
+      for (int kb = s.kb0; kb < s.kb1; ++kb, rr.next()) {
         ok = mbar_wait(bar_rempty(rr.slot), rr.phase ^ 1u, abort_flag, kStatusTimeoutWgradProducer);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
         }
-        if (lane == 0) {
-          mbar_arrive_expect_tx(bar_rfull(rr.slot), S::kRawBytes);
-          tma_load_2d(slot_raw(rr.slot), &p.q, bar_rfull(rr.slot), nc, kb * BK);
-        }
-        // codes outside the checkpoint become 0: their values are 0 as well
 #pragma unroll
-        for (int t = 0; t < BK / 32; ++t) {
-          const int k = t * 32 + lane, r = kb * BK + k;
-          const bool r_ok = c_ok && r < p.rows;
-          cp_async4(slot_codes(rr.slot) + 4 * k,
-                    p.codes + (r_ok ? static_cast<int64_t>(r) * p.lde + nc / kGroup : 0), r_ok);
-        }
+        for (int t = 0; t < BK; t += 32, r += 32, src += 32 * p.lde)
+          cp_async4(slot_codes(rr.slot) + 4 * (t + lane), r < rows ? src : p.codes, r < rows);
         cp_async_arrive(bar_rfull(rr.slot));
-        rr.next();
       }
       it.next(s);
     }
-    // the converters have read every slot
-    for (int i = 0; i < S::kRawStages && ok; ++i, rr.next())
-      ok = mbar_wait(bar_rempty(rr.slot), rr.phase ^ 1u, abort_flag, kStatusTimeoutWgradProducer);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
   } else if (warp == 1) {
@@ -522,10 +565,10 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
       const bool elected = elect_one();
       WgRing<S::kAStages> ra;
       WgRing<S::kBStages> rb;
-      WgRing<S::kDone> rd;
+      WgRing<S::kRing> rf;
       int home = 0;
       uint32_t uses0 = 0, uses1 = 0;  // chains that ran in each accumulator
-      bool ok = true;
+      bool ok = true, ready = false;
       const uint64_t a_desc = umma_desc(slot_a(0), kChunkBytes, Swz::kSbo, Swz::kLayout);
       const uint64_t b_desc = umma_desc(slot_b(0), kChunkBytes, Swz::kSbo, Swz::kLayout);
       for (WgIter it(p, worker); it.valid() && ok; home ^= 1) {
@@ -541,17 +584,25 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
           }
           tc_fence_after();
           const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kWgTileN);
+          uint32_t accumulate = 0;
           for (int kb = begin; kb < end; ++kb) {
-            ok = mbar_wait(bar_afull(ra.slot), ra.phase, abort_flag, kStatusTimeoutWgradMma) &&
-                 mbar_wait(bar_bfull(rb.slot), rb.phase, abort_flag, kStatusTimeoutWgradMma);
-            if (!__all_sync(0xffffffffu, ok)) {
-              ok = false;
-              break;
+            if (!ready) {
+              ok = mbar_wait(bar_full(rf.slot), rf.phase, abort_flag, kStatusTimeoutWgradMma);
+              if (!__all_sync(0xffffffffu, ok)) {
+                ok = false;
+                break;
+              }
             }
             tc_fence_after();
             // the start address is in units of 16 bytes in the lowest bits
             const uint64_t a0 = a_desc + static_cast<uint32_t>(ra.slot) * (PLANES * S::kABytes / 16);
             const uint64_t b0 = b_desc + static_cast<uint32_t>(rb.slot) * (S::kBBytes / 16);
+            const uint32_t done = bar_done(rf.slot);
+            ra.next();
+            rb.next();
+            rf.next();
+            // asked before the MMAs are issued: the answer arrives meanwhile
+            ready = mbar_test_wait(bar_full(rf.slot), rf.phase);
             if (elected) {
 #pragma unroll
               for (int ks = 0; ks < BK / 16; ++ks) {
@@ -559,14 +610,12 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
                 for (int j = PLANES - 1; j >= 0; --j)  // smallest plane first
                   umma_bf16_pair(d_tmem, a0 + (j * S::kABytes + ks * Swz::kMnStepBytes) / 16,
                                  b0 + ks * Swz::kMnStepBytes / 16, kIdesc,
-                                 (kb > begin || ks > 0 || j < PLANES - 1) ? 1u : 0u);
+                                 ks > 0 || j < PLANES - 1 ? 1u : accumulate);
               }
-              umma_commit_pair(bar_done(rd.slot), 0x3);
+              umma_commit_pair(done, 0x3);
             }
-            __syncwarp();
-            ra.next();
-            rb.next();
-            rd.next();
+            accumulate = 1;
+            ready = __all_sync(0xffffffffu, ready);
           }
           if (ok && elected) umma_commit_pair(bar_tfull(acc), 0x3);
           __syncwarp();
@@ -578,12 +627,13 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
       if (ok) mbar_wait(bar_tempty(1), (uses1 & 1) ^ 1u, abort_flag, kStatusTimeoutWgradMma);
       __syncwarp();
     }
-  } else if (warp < 2 + kWgEpiWarps) {
+  } else if (warp >= kWgEpiWarp0 && warp < kWgConvWarp0) {
     // ------------------------------------------------------------ epilogue
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWgEpiRegs));
     const int quarter = warp & 3;           // TMEM lanes this warp may access
-    const int half = (warp - 2) >> 2;       // its 128 of the tile's 256 columns
+    const int half = (warp - kWgEpiWarp0) >> 2;       // its 128 of the tile's 256 columns
     const uint32_t tempty0 = mapa_shared(bar_tempty(0), 0);
-    float* stg = reinterpret_cast<float*>(smem + S::kOffStaging) + (warp - 2) * 32 * 17;
+    float* stg = reinterpret_cast<float*>(smem + S::kOffStaging) + (warp - kWgEpiWarp0) * 32 * 9;
     auto release = [&](int acc) {
       tc_fence_before();
       __syncwarp();
@@ -613,6 +663,22 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
         }
         tc_fence_after();
         if (first && !last) continue;  // stays in the home accumulator
+        if (!last) {
+          // home += other, 32 columns at a time
+#pragma unroll 1
+          for (int col = kWgTileN / 2 * half; col < kWgTileN / 2 * (half + 1); col += 32) {
+            uint32_t r[32], x[32];
+            tmem_ld_32x32(t_other + col, x);
+            tmem_ld_32x32(t_home + col, r);
+            tmem_wait_ld();
+            if (col == kWgTileN / 2 * (half + 1) - 32) release(home ^ 1);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) + __uint_as_float(x[c]));
+            tmem_st_32x32(t_home + col, r);
+          }
+          tmem_wait_st();
+          continue;
+        }
         constexpr int kSteps = kWgTileN / 2 / 16;  // 16 columns each
 #pragma unroll 1
         for (int i = 0; i < kSteps; ++i) {
@@ -629,10 +695,6 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
           } else {
             tmem_wait_ld();
           }
-          if (!last) {
-            tmem_st_32x16(t_home + col, r);
-            continue;
-          }
           if (i == kSteps - 1) release(home);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {  // the converters' column order back to the result's
@@ -647,19 +709,22 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
                   make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
           } else {
 #pragma unroll
-            for (int c = 0; c < 16; ++c) stg[lane * 17 + c] = __uint_as_float(r[c]);
-            __syncwarp();
-            store_block<16>(static_cast<OUT*>(p.out), p.d_in, row0, colt + col, p.d_out, p.d_in, stg, lane,
-                            p.vec_out != 0);
-            __syncwarp();
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+              for (int c = 0; c < 8; ++c) stg[lane * 9 + c] = __uint_as_float(r[8 * h + c]);
+              __syncwarp();
+              store_block<8>(static_cast<OUT*>(p.out), p.d_in, row0, colt + col + 8 * h, p.d_out, p.d_in, stg, lane,
+                             p.vec_out != 0);
+              __syncwarp();
+            }
           }
         }
-        if (!last) tmem_wait_st();
       }
       it.next(s);
     }
-  } else {
+  } else if (warp >= kWgConvWarp0) {
     // ---------------------------------------------------------- converters
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWgConvRegs));
     // Groups of warps take k-blocks in turn, so that one group's latency hides
     // behind the other's.  A task is 16 columns of one token.  8 neighbouring
     // lanes hold 4 tasks of token k in one 64-column chunk and 4 of token k ^ 1
@@ -669,23 +734,25 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
     constexpr int kTasks = BK * 8 / (32 * kGroupWarps);
     constexpr int kTaskRows = 4 * kGroupWarps;  // tokens of one task round, a multiple of the swizzle's 8
     static_assert(kTaskRows % 8 == 0 && kTasks * kTaskRows == BK, "whole task rounds");
-    const int group = (warp - 2 - kWgEpiWarps) / kGroupWarps;
-    const int k0 = ((warp - 2 - kWgEpiWarps) % kGroupWarps) * 4 + (lane >> 4) * 2 + ((lane >> 2) & 1);
+    const int group = (warp - kWgConvWarp0) / kGroupWarps;
+    const int k0 = ((warp - kWgConvWarp0) % kGroupWarps) * 4 + (lane >> 4) * 2 + ((lane >> 2) & 1);
     const int chunk = ((lane >> 3) ^ k0) & 1, seg = lane & 3;
     const uint32_t in_off = k0 * 128 + chunk * 64 + seg * 16;
     const uint32_t out_off = chunk * kChunkBytes + k0 * 128;
     const uint32_t off0 = out_off + (((2 * seg) ^ (k0 & 7)) << 4), off1 = out_off + (((2 * seg + 1) ^ (k0 & 7)) << 4);
     const uint32_t code_off = 4 * k0 + 2 * chunk + (seg >> 1);
-    const uint32_t bfull0 = mapa_shared(bar_bfull(0), 0);
+    const uint32_t full0 = mapa_shared(bar_full(0), 0);
     WgRing<S::kRawStages> rr;
     WgRing<S::kBStages> rb;
-    WgRing<S::kDone> rd;  // the k-block kBStages back
+    WgRing<S::kRing> rf, rd;  // this k-block, and the one kBStages back (from there on)
     // k-blocks of this worker: its share and its whole tiles
     const int64_t whole = p.shared + worker < p.tiles ? (p.tiles - 1 - p.shared - worker) / p.workers + 1 : 0;
     const int64_t blocks = wgrad_begin(p, worker + 1) - wgrad_begin(p, worker) + whole * p.kblocks;
-    for (int64_t i = 0; i < blocks; ++i, rr.next(), rb.next()) {
-      if (i > S::kBStages) rd.next();
-      if (kWgConvGroups > 1 && i % kWgConvGroups != group) continue;
+    rr.slot = rb.slot = rf.slot = rd.slot = group;
+    constexpr int kSkip = kWgConvGroups;
+    static_assert(kSkip <= S::kBStages, "a group's first k-block finds its slot empty");
+    for (int64_t i = group; i < blocks; i += kSkip, rr.template skip<kSkip>(), rb.template skip<kSkip>(),
+                 rf.template skip<kSkip>()) {
       bool ok = mbar_wait(bar_rfull(rr.slot), rr.phase, abort_flag, kStatusTimeoutWgradConvert);
       if (!__all_sync(0xffffffffu, ok)) break;
       uint4 w[kTasks];
@@ -700,6 +767,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
       if (i >= S::kBStages) {
         ok = mbar_wait(bar_done(rd.slot), rd.phase, abort_flag, kStatusTimeoutWgradConvert);
         if (!__all_sync(0xffffffffu, ok)) break;
+        rd.template skip<kSkip>();
       }
 #pragma unroll
       for (int t = 0; t < kTasks; ++t) {
@@ -721,7 +789,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
       // of 614 for 16384 x 2048 x 8192).
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive_remote(bfull0 + 8u * rb.slot);
+      if (lane == 0) mbar_arrive_remote(full0 + 8u * rf.slot);
     }
   }
 
