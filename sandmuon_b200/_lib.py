@@ -181,7 +181,8 @@ def ensure_device(device: torch.device) -> None:
 
 
 def stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The device's current stream, without building a torch.cuda.Stream (2 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
 IPC_HANDLE_BYTES = 64

@@ -4,7 +4,7 @@ Between a forward and a backward pass, training holds the input of every
 linear layer for the weight gradient and the input of every activation
 function for its derivative.  This module holds them in 8 bits:
 
-    packed = pack(x)                    # int8 values, one power-of-two scale per 32 columns
+    packed = pack_input(x)              # int8 values, one power-of-two scale per 32 columns
     q, k, v = (linear(x, w, packed=packed) for w in (wq, wk, wv))   # one checkpoint, three layers
     y, packed_y = gelu(h, pack_output=True)                         # h and y held in 8 bits
     out = linear(y, w2, packed=packed_y)
@@ -28,7 +28,8 @@ from torch import nn
 
 from . import _lib, engine
 
-__all__ = ["PackedActivation", "PackedLinear", "gelu", "gelu_backward", "linear", "pack", "unpack", "weight_gradient"]
+__all__ = ["PackedActivation", "PackedLinear", "gelu", "gelu_backward", "linear", "pack", "pack_input", "unpack",
+           "weight_gradient"]
 
 
 class PackedActivation:
@@ -124,25 +125,28 @@ def weight_gradient(delta: torch.Tensor, packed: PackedActivation, *,
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, packed):
-        ctx.save_for_backward(weight, packed.values, packed.exponents)
-        ctx.packed = (packed.shape, packed.dtype)
-        ctx.x_shape, ctx.dtype = x.shape, x.dtype
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        return torch.nn.functional.linear(x, weight.to(x.dtype), None if bias is None else bias.to(x.dtype))
+        dtype = x.dtype
+        cast = weight if weight.dtype == dtype else weight.to(dtype)
+        ctx.save_for_backward(cast, packed.values, packed.exponents)
+        ctx.x_shape, ctx.weight_dtype = x.shape, weight.dtype
+        if bias is None:
+            return torch.nn.functional.linear(x, cast)
+        ctx.bias_dtype = bias.dtype
+        return torch.nn.functional.linear(x, cast, bias.to(dtype))
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, delta):
-        weight, values, exponents = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        cast, values, exponents = ctx.saved_tensors
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
         rows = _flat(delta)
         dx = dw = db = None
         if need_x:
-            dx = torch.matmul(rows, weight.to(ctx.dtype)).view(ctx.x_shape)
+            dx = torch.mm(rows, cast).view(ctx.x_shape)
         if need_w:
-            dw = engine.weight_gradient(rows, values, exponents, ctx.packed[0][-1], weight.dtype)
+            dw = engine.weight_gradient(rows, values, exponents, ctx.x_shape[-1], ctx.weight_dtype)
         if need_b:
-            sums = torch.zeros((2, rows.shape[1]), dtype=torch.float32, device=rows.device)
+            sums = rows.new_zeros((2, rows.shape[1]), dtype=torch.float32)
             engine.accumulate_column_stats(rows, sums[0], sums[1])
             db = sums[1].to(ctx.bias_dtype)
         return dx, dw, db, None
@@ -153,10 +157,11 @@ def _compute_dtype(x: torch.Tensor) -> torch.dtype:
     return torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
 
 
-def _pack_for(x: torch.Tensor, dtype: torch.dtype, stats: bool) -> PackedActivation:
-    """The checkpoint of a layer that reads x and computes in `dtype`: of x as
-    it comes, unless float16 cotangents will meet it."""
-    return pack(x.to(dtype) if dtype == torch.float16 else x, stats=stats)
+def pack_input(x: torch.Tensor, *, stats: bool = False) -> PackedActivation:
+    """The checkpoint that linear layers reading x take under the current
+    autocast state: of x as it comes, or of its float16 values where the layers
+    compute in float16 (their cotangents then need those)."""
+    return pack(x.to(torch.float16) if _compute_dtype(x) == torch.float16 else x, stats=stats)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -184,11 +189,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         if dtype == torch.float16 and packed.dtype != torch.float16:
             raise TypeError(f"a float16 layer needs a checkpoint of float16 values; got {packed.dtype}")
     if not (torch.is_grad_enabled() and weight.requires_grad):
-        # nothing reads the checkpoint: the weight keeps x out of the graph
+        # nothing reads the checkpoint, and torch's own layer keeps no x
         return torch.nn.functional.linear(x.to(dtype), weight.to(dtype), None if bias is None else bias.to(dtype))
     if packed is None:
-        packed = _pack_for(x, dtype, False)
-    return _Linear.apply(x.to(dtype), weight, bias, packed)
+        packed = pack_input(x)
+    return _Linear.apply(x if x.dtype == dtype else x.to(dtype), weight, bias, packed)
 
 
 class PackedLinear(nn.Linear):

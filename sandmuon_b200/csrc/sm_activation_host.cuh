@@ -26,7 +26,7 @@ struct ActLaunch {
 };
 
 // CTAs of 256 threads: strips of up to 256 columns times enough row ranges for
-// four CTAs per SM, each of at least two passes over its rows.
+// four CTAs per SM, each of at least four passes over its rows.
 static ActLaunch act_launch(int64_t rows, int64_t cols, bool vec, int sms) {
   ActLaunch l;
   const int64_t padded = act_lde(cols) * kGroup;
@@ -37,7 +37,7 @@ static ActLaunch act_launch(int64_t rows, int64_t cols, bool vec, int sms) {
   const int64_t row_lanes = kActThreads >> log_lanes;
   const int64_t per_pass = row_lanes * kActUnroll;
   const int64_t want = std::max<int64_t>(1, cdiv(4 * static_cast<int64_t>(sms), strips));
-  const int64_t most = std::max<int64_t>(1, cdiv(rows, 2 * per_pass));
+  const int64_t most = std::max<int64_t>(1, cdiv(rows, 4 * per_pass));
   int64_t splits = std::min<int64_t>(std::min(want, most), 65535);
   const int64_t rows_per_cta = round_up(cdiv(rows, splits), row_lanes);
   splits = std::max<int64_t>(1, cdiv(rows, rows_per_cta));

@@ -23,6 +23,11 @@ def _stream(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(_lib.stream_handle(device))
 
 
+def _on(device: torch.device):
+    """Makes `device` current; free when it already is."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 # ----------------------------------------------------------------- workspaces
 
 class _Workspaces:
@@ -69,7 +74,7 @@ def accumulate_column_stats(rows: torch.Tensor, sum_sq: torch.Tensor, total: tor
     if n_rows == 0 or n_cols == 0:
         return
     lib = _lib.load()
-    with torch.cuda.device(device):
+    with _on(device):
         nbytes = lib.sm_stats_workspace_bytes(n_rows, n_cols)
         ws = _workspaces.get(device, nbytes, "stats")
         rc = lib.sm_stats_accumulate(_ptr(rows), _lib.DTYPE_CODES[rows.dtype], n_rows, n_cols, rows.stride(0),
@@ -359,11 +364,6 @@ def _gelu_form(approximate: str) -> int:
     return form
 
 
-def _on(device: torch.device):
-    """Makes `device` current; free when it already is."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
 def _rows_2d(t: torch.Tensor, what: str) -> torch.Tensor:
     if t.dim() != 2:
         raise ValueError(f"{what} must be 2-D [rows, columns]; got {tuple(t.shape)}")
@@ -371,18 +371,18 @@ def _rows_2d(t: torch.Tensor, what: str) -> torch.Tensor:
     return t
 
 
-def new_checkpoint(rows: int, cols: int, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
-    """Uninitialised (values, exponents) of a [rows, cols] activation."""
-    return (torch.empty((rows, activation_ld(cols)), dtype=torch.int8, device=device),
-            torch.empty((rows, activation_lde(cols)), dtype=torch.uint8, device=device))
+def _new_checkpoint(like: torch.Tensor, rows: int, cols: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Uninitialised (values, exponents) of a [rows, cols] activation on `like`'s device."""
+    return (like.new_empty((rows, activation_ld(cols)), dtype=torch.int8),
+            like.new_empty((rows, activation_lde(cols)), dtype=torch.uint8))
 
 
-def _sums_buffers(rows: int, cols: int, device: torch.device):
+def _sums_buffers(like: torch.Tensor, rows: int, cols: int):
     """(result [2, cols], workspace or None, its bytes); the workspace belongs
     to one call, so captured graphs and streams never share it."""
     nbytes = _lib.load().sm_activation_sums_workspace_bytes(rows, cols)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    return torch.empty((2, cols), dtype=torch.float32, device=device), ws, nbytes
+    ws = like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    return like.new_empty((2, cols), dtype=torch.float32), ws, nbytes
 
 
 def pack_activations(rows: torch.Tensor, stats: bool = False):
@@ -392,8 +392,8 @@ def pack_activations(rows: torch.Tensor, stats: bool = False):
     device = rows.device
     n, c = rows.shape
     with _on(device):
-        values, exponents = new_checkpoint(n, c, device)
-        sums, ws, nbytes = _sums_buffers(n, c, device) if stats else (None, None, 0)
+        values, exponents = _new_checkpoint(rows, n, c)
+        sums, ws, nbytes = _sums_buffers(rows, n, c) if stats else (None, None, 0)
         rc = _lib.load().sm_activation_pack(
             rows.data_ptr(), code, n, c, rows.stride(0), rows.stride(1), values.data_ptr(), exponents.data_ptr(),
             0 if sums is None else sums.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes,
@@ -409,7 +409,7 @@ def unpack_activations(values: torch.Tensor, exponents: torch.Tensor, cols: int,
     _lib.ensure_device(device)
     n = values.shape[0]
     with _on(device):
-        out = torch.empty((n, cols), dtype=dtype, device=device)
+        out = values.new_empty((n, cols), dtype=dtype)
         rc = _lib.load().sm_activation_unpack(values.data_ptr(), exponents.data_ptr(), n, cols, out.data_ptr(), code,
                                               _lib.stream_handle(device))
     _lib.check(rc, "sm_activation_unpack")
@@ -423,10 +423,10 @@ def gelu_forward(rows: torch.Tensor, approximate: str, keep_input: bool, pack_ou
     device = rows.device
     n, c = rows.shape
     with _on(device):
-        y = torch.empty((n, c), dtype=rows.dtype, device=device)
-        kept = new_checkpoint(n, c, device) if keep_input else None
-        packed = new_checkpoint(n, c, device) if pack_output else None
-        sums, ws, nbytes = _sums_buffers(n, c, device) if pack_output and stats else (None, None, 0)
+        y = rows.new_empty((n, c))
+        kept = _new_checkpoint(rows, n, c) if keep_input else None
+        packed = _new_checkpoint(rows, n, c) if pack_output else None
+        sums, ws, nbytes = _sums_buffers(rows, n, c) if pack_output and stats else (None, None, 0)
         rc = _lib.load().sm_gelu_forward(
             rows.data_ptr(), code, n, c, rows.stride(0), rows.stride(1), form, y.data_ptr(),
             kept[0].data_ptr() if keep_input else 0, kept[1].data_ptr() if keep_input else 0,
@@ -445,7 +445,7 @@ def gelu_backward(delta: torch.Tensor, values: torch.Tensor, exponents: torch.Te
     device = delta.device
     n, c = delta.shape
     with _on(device):
-        out = torch.empty((n, c), dtype=delta.dtype, device=device)
+        out = delta.new_empty((n, c))
         rc = _lib.load().sm_gelu_backward(delta.data_ptr(), code, n, c, delta.stride(0), delta.stride(1),
                                           values.data_ptr(), exponents.data_ptr(), form, out.data_ptr(),
                                           _lib.stream_handle(device))
@@ -463,10 +463,10 @@ def weight_gradient(delta: torch.Tensor, values: torch.Tensor, exponents: torch.
     n, d_out = delta.shape
     lib = _lib.load()
     with _on(device):
-        out = torch.empty((d_out, d_in), dtype=dtype, device=device)
+        out = delta.new_empty((d_out, d_in), dtype=dtype)
         args = (delta.data_ptr(), code, n, d_out, delta.stride(0), delta.stride(1))
         nbytes = lib.sm_weight_gradient_workspace_bytes(*args, d_in)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        ws = delta.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         rc = lib.sm_weight_gradient(*args, values.data_ptr(), exponents.data_ptr(), d_in, out.data_ptr(), out_code,
                                     0 if ws is None else ws.data_ptr(), nbytes, _lib.stream_handle(device))
     _lib.check(rc, "sm_weight_gradient")

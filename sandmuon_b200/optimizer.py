@@ -15,12 +15,30 @@ import torch
 from torch import nn
 from torch.optim import Optimizer
 
-from . import _lib, engine
+from . import _lib, activations, engine
 from .coefficients import S8_COEFFICIENTS, S8_MARGIN, S8_MULTIPLIER
 from .functional import (_graft_direction, _s8_fp32, diagonal_inverse_sqrt, rank1_inverse_sqrt,  # noqa: F401
                          rank1_mapback, rank1_whiten)
 
 _QKV_SHARING = re.compile(r"^(transformer\.h\.\d+\.attn\.)[kv]_proj\.weight$")
+
+
+def _packed_input(module, inputs, keywords):
+    """The checkpoint a PackedLinear was called with, else None."""
+    if not isinstance(module, activations.PackedLinear):
+        return None
+    return inputs[1] if len(inputs) > 1 else keywords.get("packed")
+
+
+def _pack_with_sums(module, inputs, keywords):
+    """Forward pre-hook of a PackedLinear whose input statistics are wanted:
+    packs the input with its column sums, so that the forward hook need not
+    read the input again."""
+    x = inputs[0] if inputs else None
+    if (module.training and torch.is_grad_enabled() and module.weight.requires_grad and isinstance(x, torch.Tensor)
+            and _packed_input(module, inputs, keywords) is None):
+        return inputs[:1], {"packed": activations.pack_input(x, stats=True)}
+    return None
 
 
 class DiagonalWeightedPE(Optimizer):
@@ -104,13 +122,16 @@ class DiagonalWeightedPE(Optimizer):
         self.handles = []
         for name, module in modules.items():
             parameter = matrices[name]
-            self.handles.append(module.register_forward_hook(
-                self._capture(parameter, capture_a=self.a_sources[id(parameter)] is parameter)))
+            capture_a = self.a_sources[id(parameter)] is parameter
+            if capture_a and isinstance(module, activations.PackedLinear):
+                self.handles.append(module.register_forward_pre_hook(_pack_with_sums, with_kwargs=True))
+            self.handles.append(module.register_forward_hook(self._capture(parameter, capture_a=capture_a),
+                                                             with_kwargs=True))
 
     # ------------------------------------------------------------- hooks
 
     def _capture(self, parameter, *, capture_a):
-        def hook(module, inputs, output):
+        def hook(module, inputs, keywords, output):
             if (not module.training or not torch.is_grad_enabled() or
                     not isinstance(output, torch.Tensor) or not output.requires_grad):
                 return
@@ -123,8 +144,14 @@ class DiagonalWeightedPE(Optimizer):
                     state["a_count"] = 0
                     if self.rank_one_a:
                         state["a_first_sum"] = self._stat_slot(parameter, "a_first_sum", rows.shape[-1], rows.device)
-                engine.accumulate_column_stats(rows, state["a_sum"],
-                                               state["a_first_sum"] if self.rank_one_a else None)
+                first_sum = state["a_first_sum"] if self.rank_one_a else None
+                packed = _packed_input(module, inputs, keywords)
+                if packed is None or packed.sums is None:
+                    engine.accumulate_column_stats(rows, state["a_sum"], first_sum)
+                elif first_sum is None:
+                    state["a_sum"].add_(packed.sums[0])
+                else:
+                    torch._foreach_add_([state["a_sum"], first_sum], [packed.sums[0], packed.sums[1]])
                 state["a_count"] += rows.shape[0]
 
             def cotangent_hook(gradient):

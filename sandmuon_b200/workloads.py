@@ -12,6 +12,8 @@ import numpy as np
 import torch
 from torch import nn
 
+from . import activations
+
 
 def gpt_matrix_model(layers: int, width: int, hidden: int) -> nn.Module:
     """Module tree with the historical GPT names (q/k/v/o, mlp.c_fc, mlp.c_proj)
@@ -104,36 +106,54 @@ def s8_dense_flops(shapes) -> float:
 
 # ------------------------------------------------------------ config 2: GPT-2
 
-class CausalSelfAttention(nn.Module):
-    """Bias-free q/k/v/o projections around torch's fused causal attention."""
+def _linear_class(checkpoints: str | None) -> type[nn.Linear]:
+    """nn.Linear, or the layer that holds its input in 8 bits ("int8")."""
+    if checkpoints not in (None, "int8"):
+        raise ValueError(f'checkpoints must be None or "int8"; got {checkpoints!r}')
+    return nn.Linear if checkpoints is None else activations.PackedLinear
 
-    def __init__(self, width: int, heads: int):
+
+class CausalSelfAttention(nn.Module):
+    """Bias-free q/k/v/o projections around torch's fused causal attention.
+    checkpoints="int8": q, k and v share one 8-bit checkpoint of their input."""
+
+    def __init__(self, width: int, heads: int, checkpoints: str | None = None):
         super().__init__()
         self.heads = heads
+        self.checkpoints = checkpoints
+        linear = _linear_class(checkpoints)
         for proj in ("q_proj", "k_proj", "v_proj", "o_proj"):
-            setattr(self, proj, nn.Linear(width, width, bias=False))
+            setattr(self, proj, linear(width, width, bias=False))
 
     def forward(self, x):
         b, t, c = x.shape
-        q, k, v = (p(x).view(b, t, self.heads, c // self.heads).transpose(1, 2)
+        packed = ()
+        if self.checkpoints and self.training and torch.is_grad_enabled():
+            packed = (activations.pack_input(x, stats=True),)
+        q, k, v = (p(x, *packed).view(b, t, self.heads, c // self.heads).transpose(1, 2)
                    for p in (self.q_proj, self.k_proj, self.v_proj))
         y = torch.nn.functional.scaled_dot_product_attention(q, k, v, is_causal=True)
         return self.o_proj(y.transpose(1, 2).reshape(b, t, c))
 
 
 class GPT2Block(nn.Module):
-    def __init__(self, width: int, heads: int, hidden: int):
+    def __init__(self, width: int, heads: int, hidden: int, checkpoints: str | None = None):
         super().__init__()
+        self.checkpoints = checkpoints
+        linear = _linear_class(checkpoints)
         self.ln_1 = nn.LayerNorm(width)
-        self.attn = CausalSelfAttention(width, heads)
+        self.attn = CausalSelfAttention(width, heads, checkpoints)
         self.ln_2 = nn.LayerNorm(width)
         self.mlp = nn.Module()
-        self.mlp.c_fc = nn.Linear(width, hidden, bias=False)
-        self.mlp.c_proj = nn.Linear(hidden, width, bias=False)
+        self.mlp.c_fc = linear(width, hidden, bias=False)
+        self.mlp.c_proj = linear(hidden, width, bias=False)
 
     def forward(self, x):
         x = x + self.attn(self.ln_1(x))
-        return x + self.mlp.c_proj(torch.nn.functional.gelu(self.mlp.c_fc(self.ln_2(x))))
+        h = self.mlp.c_fc(self.ln_2(x))
+        if self.checkpoints and self.training and torch.is_grad_enabled():
+            return x + self.mlp.c_proj(*activations.gelu(h, pack_output=True, stats=True))
+        return x + self.mlp.c_proj(torch.nn.functional.gelu(h))
 
 
 class GPT2(nn.Module):
@@ -142,15 +162,17 @@ class GPT2(nn.Module):
     blocks of bias-free Linear layers, final LayerNorm, and an output head
     tied to the token embedding.  Random initialisation (N(0, 0.02^2)); the
     SandMuon matrices are the transformer.h.* Linear weights, everything else
-    (embeddings, LayerNorms) trains with the AdamW auxiliaries."""
+    (embeddings, LayerNorms) trains with the AdamW auxiliaries.
+    checkpoints="int8" holds the inputs of the block's Linear layers and GELUs
+    in 8 bits between forward and backward (sandmuon_b200.activations)."""
 
     def __init__(self, layers: int = 9, width: int = 768, heads: int = 12, vocab: int = 50257,
-                 context: int = 1024):
+                 context: int = 1024, checkpoints: str | None = None):
         super().__init__()
         self.transformer = nn.Module()
         self.transformer.wte = nn.Embedding(vocab, width)
         self.transformer.wpe = nn.Embedding(context, width)
-        self.transformer.h = nn.ModuleList([GPT2Block(width, heads, 4 * width) for _ in range(layers)])
+        self.transformer.h = nn.ModuleList([GPT2Block(width, heads, 4 * width, checkpoints) for _ in range(layers)])
         self.transformer.ln_f = nn.LayerNorm(width)
         for name, p in self.named_parameters():
             if p.ndim == 2:

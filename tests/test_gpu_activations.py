@@ -139,7 +139,7 @@ def test_weight_gradient(rows, d_in, d_out, dtype, out_dtype):
 
 def check_weight_gradient(got, delta, packed, out_dtype=torch.float32):
     d = f64(delta).reshape(-1, delta.shape[-1])
-    hat = f64(packed.unpack(torch.float32)).reshape(d.shape[0], -1)
+    hat = f64(packed.unpack(torch.float32)).reshape(d.shape[0], packed.shape[-1])
     want, size = d.T @ hat, np.abs(d).T @ np.abs(hat)
     bound = (d.shape[0] + 64) * 3 * 2.0 ** -23 * size + half_step(out_dtype) * np.abs(want)
     if out_dtype == torch.float16:
