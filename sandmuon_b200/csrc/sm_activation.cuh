@@ -265,16 +265,23 @@ __device__ __forceinline__ void store_strided(T* y, int64_t r, int64_t col0, int
 }
 
 // x^ of 8 consecutive values, exactly: u = q + 128 in the low mantissa bits of
-// 2^23, (2^23 + u) - (2^23 + 128) = q.
+// 2^23, ((2^23 + u) - (2^23 + 128)) * 2^e = q * 2^e, in one fused step while
+// 2^23 * 2^e is finite.
 constexpr float kByteBias = 8388608.0f + 128.0f;
+constexpr uint32_t kFusedCodes = 127 + 100;
 
 __device__ __forceinline__ void unpack8(uint2 w, uint32_t code, float (&v)[8]) {
-  const float s = code_scale(code);
   const uint32_t u[2] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t f = __byte_perm(u[i / 4], 0x4b000000u, 0x7650u | (i & 3));
-    v[i] = (__uint_as_float(f) - kByteBias) * s;
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(__byte_perm(u[i / 4], 0x4b000000u, 0x7650u | (i & 3)));
+  if (code <= kFusedCodes) {
+    const float s = __uint_as_float(code << 23), bias = -kByteBias * s;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], s, bias);
+  } else {
+    const float s = code_scale(code);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (v[i] - kByteBias) * s;
   }
 }
 
@@ -348,31 +355,39 @@ __device__ __forceinline__ void write_column_sums(const ActGeometry& g, const Ac
 }
 
 // sums[j] = sum over splits of partials[s][j], j < n = 2 * cols, in a fixed
-// order: 32 columns x 8 split lanes per CTA, FP64.
-__global__ void __launch_bounds__(256) k_column_sums_finish(const float* __restrict__ partials, int64_t n, int splits,
-                                                            float* __restrict__ sums) {
-  __shared__ double sh[8][33];
+// order: 32 columns x 32 split lanes per CTA (all loads of a few hundred splits
+// in flight at once), FP64.
+constexpr int kFinishLanes = 32;
+
+__global__ void __launch_bounds__(32 * kFinishLanes)
+    k_column_sums_finish(const float* __restrict__ partials, int64_t n, int splits, float* __restrict__ sums) {
+  __shared__ double sh[kFinishLanes][33];
   const int c = threadIdx.x & 31, l = threadIdx.x >> 5;
   const int64_t j = static_cast<int64_t>(blockIdx.x) * 32 + c;
   grid_dep_wait();
   double s = 0.0;
   if (j < n) {
 #pragma unroll 8
-    for (int k = l; k < splits; k += 8) s += static_cast<double>(partials[static_cast<int64_t>(k) * n + j]);
+    for (int k = l; k < splits; k += kFinishLanes) s += static_cast<double>(partials[static_cast<int64_t>(k) * n + j]);
   }
   sh[l][c] = s;
   __syncthreads();
-  if (l == 0 && j < n) {
-#pragma unroll
-    for (int k = 1; k < 8; ++k) s += sh[k][c];
-    sums[j] = static_cast<float>(s);
-  }
+  // warp l joins column l of the block, its lanes the split lanes
+  const int64_t out = static_cast<int64_t>(blockIdx.x) * 32 + l;
+  s = warp_sum_d(sh[c][l]);
+  if (c == 0 && out < n) sums[out] = static_cast<float>(s);
 }
 
 // --------------------------------------------------------------- the kernels
 
-// Rows in flight per lane: enough loads to cover HBM latency at 8 warps a CTA.
+// Rows in flight per lane, and CTAs resident on an SM: a launch is one wave of
+// them.
 constexpr int kActUnroll = 4;
+constexpr int kPackCtas = 4, kUnpackCtas = 4, kGeluForwardCtas = 4;
+__host__ __device__ constexpr int gelu_backward_ctas(int elem_bytes) { return elem_bytes == 2 ? 6 : 4; }
+// The residency asked of the compiler; the strided mapping, bound by its
+// element accesses, is left its registers.
+__host__ __device__ constexpr int resident(bool vec, int ctas) { return vec ? ctas : 2; }
 
 // A VEC lane's walk down its rows: where its next row's 8 elements of each
 // tensor are (null where there is none), and how far apart rows it visits are.
@@ -409,7 +424,7 @@ __device__ __forceinline__ void act_rows(const ActGeometry& g, const ActLane& a,
 }
 
 template <typename T, bool VEC, bool STATS>
-__global__ void __launch_bounds__(kActThreads)
+__global__ void __launch_bounds__(kActThreads, resident(VEC, kPackCtas))
     k_activation_pack(const T* __restrict__ x, int64_t rs, int64_t cs, ActGeometry g, Checkpoint c,
                       float* __restrict__ sums) {
   const ActLane a = act_lane<VEC>(g);
@@ -417,28 +432,30 @@ __global__ void __launch_bounds__(kActThreads)
 #pragma unroll
   for (int i = 0; i < 8; ++i) sq[i] = su[i] = 0.0f;
   auto add = [&](const float(&v)[8]) {
-    if (!STATS) return;
+    if constexpr (STATS) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sq[i] = fmaf(v[i], v[i], sq[i]);
-      su[i] += v[i];
+      for (int i = 0; i < 8; ++i) {
+        sq[i] = fmaf(v[i], v[i], sq[i]);
+        su[i] += v[i];
+      }
     }
   };
   if constexpr (VEC) {
+    constexpr int kUnroll = sizeof(T) == 2 ? kActUnroll : 2;
     const bool in_x = a.col0 < g.cols, in_values = a.col0 < c.ld, in_codes = a.col0 / kGroup < c.lde;
     RowPointer<const T> xp(x, a.r_begin + a.row_lane, rs, a.col0, a.row_lanes);
     PackPointer pp(c, a);
-    act_rows<kActUnroll>(g, a, [&](auto full, int64_t r0) {
+    act_rows<kUnroll>(g, a, [&](auto full, int64_t r0) {
       constexpr bool kFull = decltype(full)::value;
-      Vec8<T> w[kActUnroll];
+      Vec8<T> w[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kActUnroll; ++u) {
+      for (int u = 0; u < kUnroll; ++u) {
         memset(&w[u], 0, sizeof(w[u]));
         const T* at = xp.take();
         if (kFull || (in_x && r0 + u * a.row_lanes + a.row_lane < a.r_end)) vec8_load(at, w[u]);
       }
 #pragma unroll
-      for (int u = 0; u < kActUnroll; ++u) {
+      for (int u = 0; u < kUnroll; ++u) {
         float v[8];
         vec8_unpack(w[u], v);
         pack8<T, kFull>(pp.values.take(), pp.codes.take(), w[u], v, r0 + u * a.row_lanes + a.row_lane < a.r_end,
@@ -459,7 +476,7 @@ __global__ void __launch_bounds__(kActThreads)
 }
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kActThreads)
+__global__ void __launch_bounds__(kActThreads, resident(VEC, kUnpackCtas))
     k_activation_unpack(ActGeometry g, Checkpoint c, T* __restrict__ out) {
   const ActLane a = act_lane<VEC>(g);
   if constexpr (VEC) {
@@ -529,7 +546,7 @@ constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 constexpr float kSqrt2OverPi = 0.79788456080286536f;
 constexpr float kGeluCubic = 0.044715f;
 
-// Phi(-|x|) and exp(-x^2 / 2)
+// Phi(-|x|) / exp(-x^2 / 2), and exp(-x^2 / 2)
 __device__ __forceinline__ float normal_tail(float x, float& density) {
   const float u = rcp_approx(fmaf(fabsf(x), 0.35f, 1.0f));
   density = ex2_approx(x * (x * (-0.5f * kLog2E)));
@@ -542,7 +559,7 @@ __device__ __forceinline__ float normal_tail(float x, float& density) {
   g = fmaf(g, u, 0.11982129f);
   g = fmaf(g, u, 0.13986352f);
   g = fmaf(g, u, 0.13962130f);
-  return density * (g * u);
+  return g * u;
 }
 
 // The logistic function of 2 sqrt(2/pi) (x + 0.044715 x^3): the tanh form is
@@ -557,8 +574,8 @@ template <bool TANH>
 __device__ __forceinline__ float gelu_value(float x) {
   if (TANH) return x * tanh_gate(x, x * x);
   float density;
-  const float h = normal_tail(x, density);
-  return fmaf(-fabsf(fminf(x, 40.0f)), h, fmaxf(x, 0.0f));
+  const float t = normal_tail(x, density);
+  return fmaf(-fabsf(fminf(x, 40.0f)), density * t, fmaxf(x, 0.0f));
 }
 
 template <bool TANH>
@@ -570,15 +587,17 @@ __device__ __forceinline__ float gelu_slope(float x) {
     const float x2 = x * x, s = tanh_gate(x, x2);
     return fmaf(s * (1.0f - s), x * fmaf(x2, 6.0f * kSqrt2OverPi * kGeluCubic, 2.0f * kSqrt2OverPi), s);
   }
+  // Phi(x) + x phi(x) = [x >= 0] + exp(-x^2 / 2) (x / sqrt(2 pi) - sign(x) t),
+  // both by x's sign bit
   float density;
-  const float h = normal_tail(x, density);
-  return fmaf(x * kInvSqrt2Pi, density, x > 0.0f ? 1.0f - h : h);
+  const float t = normal_tail(x, density);
+  return fmaf(density, fmaf(x, kInvSqrt2Pi, -copysignf(t, x)), __float_as_int(x) >= 0 ? 1.0f : 0.0f);
 }
 
 // y = gelu(x); packs x into `in` (PACK_IN) and the rounded y into `out` with
 // y's column sums (PACK_OUT; sums may be null).
 template <typename T, bool VEC, bool TANH, bool PACK_IN, bool PACK_OUT>
-__global__ void __launch_bounds__(kActThreads)
+__global__ void __launch_bounds__(kActThreads, resident(VEC, kGeluForwardCtas))
     k_gelu_forward(const T* __restrict__ x, int64_t rs, int64_t cs, ActGeometry g, T* __restrict__ y, Checkpoint in,
                    Checkpoint out, float* __restrict__ sums) {
   const ActLane a = act_lane<VEC>(g);
@@ -586,11 +605,12 @@ __global__ void __launch_bounds__(kActThreads)
 #pragma unroll
   for (int i = 0; i < 8; ++i) sq[i] = su[i] = 0.0f;
   auto add = [&](const float(&v)[8]) {
-    if (!PACK_OUT) return;
+    if constexpr (PACK_OUT) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sq[i] = fmaf(v[i], v[i], sq[i]);
-      su[i] += v[i];
+      for (int i = 0; i < 8; ++i) {
+        sq[i] = fmaf(v[i], v[i], sq[i]);
+        su[i] += v[i];
+      }
     }
   };
   if constexpr (VEC) {
@@ -647,7 +667,7 @@ __global__ void __launch_bounds__(kActThreads)
 
 // dx = delta * gelu'(x^)
 template <typename T, bool VEC, bool TANH>
-__global__ void __launch_bounds__(kActThreads)
+__global__ void __launch_bounds__(kActThreads, resident(VEC, gelu_backward_ctas(sizeof(T))))
     k_gelu_backward(const T* __restrict__ delta, int64_t rs, int64_t cs, ActGeometry g, Checkpoint c,
                     T* __restrict__ dx) {
   const ActLane a = act_lane<VEC>(g);

@@ -26,20 +26,20 @@ struct ActLaunch {
 };
 
 // CTAs of 256 threads: strips of up to 256 columns times enough row ranges for
-// four CTAs per SM, each of at least four passes over its rows.
-static ActLaunch act_launch(int64_t rows, int64_t cols, bool vec, int sms) {
+// one wave of `ctas` CTAs per SM, each range of whole passes.  Up to four
+// passes stay in one range: a second launch to join column sums costs more.
+static ActLaunch act_launch(int64_t rows, int64_t cols, bool vec, int sms, int ctas) {
   ActLaunch l;
   const int64_t padded = act_lde(cols) * kGroup;
   int log_lanes = 2;
   while (log_lanes < 5 && (int64_t{8} << log_lanes) < padded) ++log_lanes;
   if (!vec) log_lanes = 5;
   const int64_t strips = cdiv(padded, int64_t{8} << log_lanes);
-  const int64_t row_lanes = kActThreads >> log_lanes;
-  const int64_t per_pass = row_lanes * kActUnroll;
-  const int64_t want = std::max<int64_t>(1, cdiv(4 * static_cast<int64_t>(sms), strips));
-  const int64_t most = std::max<int64_t>(1, cdiv(rows, 4 * per_pass));
+  const int64_t per_pass = (kActThreads >> log_lanes) * kActUnroll;
+  const int64_t want = std::max<int64_t>(1, static_cast<int64_t>(ctas) * sms / strips);
+  const int64_t most = rows <= 4 * per_pass ? 1 : cdiv(rows, per_pass);
   int64_t splits = std::min<int64_t>(std::min(want, most), 65535);
-  const int64_t rows_per_cta = round_up(cdiv(rows, splits), row_lanes);
+  const int64_t rows_per_cta = round_up(cdiv(rows, splits), per_pass);
   splits = std::max<int64_t>(1, cdiv(rows, rows_per_cta));
   l.g.rows = rows;
   l.g.cols = cols;
@@ -88,8 +88,8 @@ static int act_sums_finish(const ActLaunch& l, const float* partials, float* sum
   if (sums == nullptr || l.splits == 1) return SM_OK;
   PdlScope pdl(true);
   const int64_t n = 2 * l.g.cols;
-  return launch_kernel(k_column_sums_finish, dim3(static_cast<unsigned>(cdiv(n, 32))), dim3(256), 0, st, partials, n,
-                       l.splits, sums);
+  return launch_kernel(k_column_sums_finish, dim3(static_cast<unsigned>(cdiv(n, 32))), dim3(32 * kFinishLanes), 0, st,
+                       partials, n, l.splits, sums);
 }
 
 template <typename T>
@@ -219,7 +219,7 @@ static int wgrad_geometry(const void* delta, int dtype, int64_t rows, int64_t d_
 }
 
 template <int PLANES, bool F16, int BK, typename OUT>
-static int wgrad_launch(const WgradArgs& p, bool partial, cudaStream_t st) {
+static int wgrad_launch(const WgradArgs& p, bool planes, bool partial, cudaStream_t st) {
   using S = WgSmem<PLANES, BK>;
   auto kern = k_wgrad<PLANES, F16, BK, OUT>;
   static bool attr_done[64] = {};
@@ -230,21 +230,25 @@ static int wgrad_launch(const WgradArgs& p, bool partial, cudaStream_t st) {
     SM_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal));
     attr_done[dev] = true;
   }
-  cudaLaunchConfig_t cfg;
-  cudaLaunchAttribute attr[2];
-  pair_launch_config(&cfg, attr, 2 * p.workers, S::kTotal, st);
-  cfg.blockDim = dim3(kWgThreads);
-  SM_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
+  {
+    // after k_wgrad_planes the prologue may overlap its end
+    PdlScope pdl(planes);
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[2];
+    pair_launch_config(&cfg, attr, 2 * p.workers, S::kTotal, st);
+    cfg.blockDim = dim3(kWgThreads);
+    SM_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
+  }
   if (!partial) return SM_OK;
   PdlScope pdl(true);
   return launch_kernel(k_wgrad_join<OUT>, dim3(static_cast<unsigned>(p.shared), 64), dim3(256), 0, st, p);
 }
 
 template <int PLANES, bool F16, int BK>
-static int wgrad_dispatch(int out_dtype, const WgradArgs& p, bool partial, cudaStream_t st) {
-  if (out_dtype == SM_DTYPE_F32) return wgrad_launch<PLANES, F16, BK, float>(p, partial, st);
-  if (out_dtype == SM_DTYPE_BF16) return wgrad_launch<PLANES, F16, BK, __nv_bfloat16>(p, partial, st);
-  return wgrad_launch<PLANES, F16, BK, __half>(p, partial, st);
+static int wgrad_dispatch(int out_dtype, const WgradArgs& p, bool planes, bool partial, cudaStream_t st) {
+  if (out_dtype == SM_DTYPE_F32) return wgrad_launch<PLANES, F16, BK, float>(p, planes, partial, st);
+  if (out_dtype == SM_DTYPE_BF16) return wgrad_launch<PLANES, F16, BK, __nv_bfloat16>(p, planes, partial, st);
+  return wgrad_launch<PLANES, F16, BK, __half>(p, planes, partial, st);
 }
 
 }  // namespace smb
@@ -258,7 +262,9 @@ size_t sm_activation_sums_workspace_bytes(int64_t n_rows, int64_t n_cols) {
   int sms = 148;
   DeviceInfo* di;
   if (current_device_info(&di) == SM_OK) sms = di->sms;
-  const int splits = std::max(act_launch(n_rows, n_cols, true, sms).splits, act_launch(n_rows, n_cols, false, sms).splits);
+  constexpr int kCtas = std::max(kPackCtas, kGeluForwardCtas);
+  const int splits = std::max(act_launch(n_rows, n_cols, true, sms, kCtas).splits,
+                              act_launch(n_rows, n_cols, false, sms, kCtas).splits);
   return splits == 1 ? 0 : static_cast<size_t>(splits) * 2 * static_cast<size_t>(n_cols) * sizeof(float);
 }
 
@@ -277,7 +283,7 @@ int sm_activation_pack(const void* x, int dtype, int64_t n_rows, int64_t n_cols,
   DeviceInfo* di;
   SM_TRY(current_device_info(&di));
   const bool vec = vec8_rows(x, dtype, n_rows, n_cols, row_stride, col_stride);
-  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms);
+  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms, kPackCtas);
   const Checkpoint c = act_checkpoint(values, exponents, n_cols);
   float* target = nullptr;
   SM_TRY(act_sums_target(l, sums, workspace, workspace_bytes, &target));
@@ -299,7 +305,7 @@ int sm_activation_unpack(const int8_t* values, const uint8_t* exponents, int64_t
   SM_TRY(current_device_info(&di));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool vec = vec8_rows(out, dtype, n_rows, n_cols, n_cols, 1);
-  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms);
+  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms, kUnpackCtas);
   const Checkpoint c = act_checkpoint(values, exponents, n_cols);
   if (dtype == SM_DTYPE_F32) return unpack_run(l, c, static_cast<float*>(out), vec, st);
   if (dtype == SM_DTYPE_BF16) return unpack_run(l, c, static_cast<__nv_bfloat16*>(out), vec, st);
@@ -325,7 +331,7 @@ int sm_gelu_forward(const void* x, int dtype, int64_t n_rows, int64_t n_cols, in
   SM_TRY(current_device_info(&di));
   const bool vec = vec8_rows(x, dtype, n_rows, n_cols, row_stride, col_stride) &&
                    vec8_rows(y, dtype, n_rows, n_cols, n_cols, 1);
-  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms);
+  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms, kGeluForwardCtas);
   const Checkpoint in = act_checkpoint(in_values, in_exponents, n_cols);
   const Checkpoint out = act_checkpoint(out_values, out_exponents, n_cols);
   float* target = nullptr;
@@ -355,7 +361,7 @@ int sm_gelu_backward(const void* delta, int dtype, int64_t n_rows, int64_t n_col
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool vec = vec8_rows(delta, dtype, n_rows, n_cols, row_stride, col_stride) &&
                    vec8_rows(dx, dtype, n_rows, n_cols, n_cols, 1);
-  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms);
+  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms, gelu_backward_ctas(elem_size(dtype)));
   const Checkpoint c = act_checkpoint(values, exponents, n_cols);
   const bool th = form == SM_GELU_TANH;
   if (dtype == SM_DTYPE_F32)
@@ -405,14 +411,19 @@ int sm_weight_gradient(const void* delta, int dtype, int64_t n_rows, int64_t d_o
   int64_t stride = std::max(row_stride, round_up(d_out, 8)) * 2;
   if (!g.direct) {
     uint16_t* planes = static_cast<uint16_t*>(workspace);
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(cdiv(plane_elems, 256), 148 * 16));
-    if (dtype == SM_DTYPE_F32)
-      SM_TRY(launch_kernel(k_wgrad_planes<float, 3>, dim3(grid), dim3(256), 0, st, static_cast<const float*>(delta),
+    const dim3 block(32, 8);
+    const int64_t strips = cdiv(g.plane_ld, 32 * 8);
+    const dim3 grid(static_cast<unsigned>(strips),
+                    static_cast<unsigned>(std::min<int64_t>(cdiv(n_rows, 8), std::max<int64_t>(1, 16 * 148 / strips))));
+    if (dtype == SM_DTYPE_F32) {
+      auto kern = vec8_rows(delta, dtype, n_rows, d_out, row_stride, col_stride) ? k_wgrad_planes<float, 3, true>
+                                                                                : k_wgrad_planes<float, 3, false>;
+      SM_TRY(launch_kernel(kern, grid, block, 0, st, static_cast<const float*>(delta), row_stride, col_stride, n_rows,
+                           d_out, g.plane_ld, planes));
+    } else {
+      SM_TRY(launch_kernel(k_wgrad_planes<__half, 1, false>, grid, block, 0, st, static_cast<const __half*>(delta),
                            row_stride, col_stride, n_rows, d_out, g.plane_ld, planes));
-    else
-      SM_TRY(launch_kernel(k_wgrad_planes<__half, 1>, dim3(grid), dim3(256), 0, st,
-                           static_cast<const __half*>(delta), row_stride, col_stride, n_rows, d_out, g.plane_ld,
-                           planes));
+    }
     base = static_cast<const uint8_t*>(workspace);
     stride = g.plane_ld * 2;
   }
@@ -430,9 +441,9 @@ int sm_weight_gradient(const void* delta, int dtype, int64_t n_rows, int64_t d_o
   p.out = out;
   p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + g.plane_bytes);
   p.vec_out = aligned(out, 16) && (d_in * elem_size(out_dtype)) % 16 == 0;
-  if (dtype == SM_DTYPE_F32) return wgrad_dispatch<3, false, 32>(out_dtype, p, g.partial, st);
-  if (dtype == SM_DTYPE_BF16) return wgrad_dispatch<1, false, 64>(out_dtype, p, g.partial, st);
-  return wgrad_dispatch<1, true, 64>(out_dtype, p, g.partial, st);
+  if (dtype == SM_DTYPE_F32) return wgrad_dispatch<3, false, 32>(out_dtype, p, !g.direct, g.partial, st);
+  if (dtype == SM_DTYPE_BF16) return wgrad_dispatch<1, false, 64>(out_dtype, p, !g.direct, g.partial, st);
+  return wgrad_dispatch<1, true, 64>(out_dtype, p, !g.direct, g.partial, st);
 }
 
 }  // extern "C"

@@ -851,30 +851,57 @@ __global__ void __launch_bounds__(256) k_wgrad_join(const __grid_constant__ Wgra
 // 8 elements, padding 0).  One plane keeps the type; three split an FP32 value
 // by truncation into BF16 parts of 8 significant bits: h + m + l == v exactly
 // (short of BF16's underflow).  inf and NaN live in the first plane alone.
-template <typename T, int PLANES>
+// A thread makes 8 columns of a plane row (16-byte stores; 16-byte loads where
+// VEC says that delta's rows allow them).
+template <typename T, int PLANES, bool VEC>
 __global__ void __launch_bounds__(256)
     k_wgrad_planes(const T* __restrict__ delta, int64_t rs, int64_t cs, int64_t rows, int64_t cols, int64_t ld,
                    uint16_t* __restrict__ planes) {
-  const int64_t n = rows * ld;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += step) {
-    const int64_t r = i / ld, c = i - r * ld;
-    if (PLANES == 1) {
-      uint16_t bits = 0;
-      if (c < cols) memcpy(&bits, &delta[r * rs + c * cs], 2);
-      planes[i] = bits;
-    } else {
-      float v = c < cols ? to_f32(delta[r * rs + c * cs]) : 0.0f;
+  const int64_t c0 = (static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x) * 8;
+  if (c0 < ld) {
+    for (int64_t r = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y; r < rows;
+         r += static_cast<int64_t>(gridDim.y) * blockDim.y) {
+      const T* src = delta + r * rs + c0 * cs;
+      uint16_t* dst = planes + r * ld + c0;
+      if constexpr (PLANES == 1) {
+        uint16_t b[8];
 #pragma unroll
-      for (int j = 0; j < PLANES; ++j) {
-        uint32_t top = __float_as_uint(v) & 0xffff0000u;
-        const bool special = (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u;
-        if (special && v != v) top |= 0x00400000u;  // NaN whatever its payload
-        planes[j * n + i] = static_cast<uint16_t>(top >> 16);
-        v = special ? 0.0f : v - __uint_as_float(top);
+        for (int i = 0; i < 8; ++i) {
+          b[i] = 0;
+          if (c0 + i < cols) memcpy(&b[i], src + i * cs, 2);
+        }
+        uint4 w;
+        memcpy(&w, b, 16);
+        *reinterpret_cast<uint4*>(dst) = w;
+      } else {
+        float v[8];
+        if constexpr (VEC) {
+          Vec8<float> w;
+          vec8_load(src, w);
+          vec8_unpack(w, v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = c0 + i < cols ? src[i * cs] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < PLANES; ++j) {
+          uint32_t top[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t bits = __float_as_uint(v[i]);
+            const bool special = (bits & 0x7f800000u) == 0x7f800000u;
+            top[i] = bits & 0xffff0000u;
+            if (special && (bits & 0x007fffffu) != 0) top[i] |= 0x00400000u;  // NaN whatever its payload
+            v[i] = special ? 0.0f : v[i] - __uint_as_float(top[i]);
+          }
+          *reinterpret_cast<uint4*>(dst + j * rows * ld) =
+              make_uint4(__byte_perm(top[0], top[1], 0x7632), __byte_perm(top[2], top[3], 0x7632),
+                         __byte_perm(top[4], top[5], 0x7632), __byte_perm(top[6], top[7], 0x7632));
+        }
       }
     }
   }
+  grid_dep_launch();
 }
 
 }  // namespace smb
