@@ -80,7 +80,8 @@ def _flat(t: torch.Tensor) -> torch.Tensor:
 
 
 def _of_shape(packed: PackedActivation, shape, what: str) -> None:
-    if packed.shape[-1] != shape[-1] or math.prod(packed.shape[:-1]) != math.prod(shape[:-1]):
+    if packed.shape != shape and (packed.shape[-1] != shape[-1]
+                                  or packed.values.shape[0] != math.prod(shape[:-1])):
         raise ValueError(f"the checkpoint of a {packed.shape} activation does not fit {what} {tuple(shape)}")
 
 
@@ -142,13 +143,15 @@ class _Linear(torch.autograd.Function):
         rows = _flat(delta)
         dx = dw = db = None
         if need_x:
-            dx = torch.mm(rows, cast).view(ctx.x_shape)
+            dx = torch.mm(rows, cast)
+            if dx.shape != ctx.x_shape:
+                dx = dx.view(ctx.x_shape)
         if need_w:
             dw = engine.weight_gradient(rows, values, exponents, ctx.x_shape[-1], ctx.weight_dtype)
         if need_b:
-            sums = rows.new_zeros((2, rows.shape[1]), dtype=torch.float32)
-            engine.accumulate_column_stats(rows, sums[0], sums[1])
-            db = sums[1].to(ctx.bias_dtype)
+            db = engine.column_sums(rows)
+            if ctx.bias_dtype != torch.float32:
+                db = db.to(ctx.bias_dtype)
         return dx, dw, db, None
 
 
@@ -179,9 +182,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         raise ValueError(f"linear: bias {tuple(bias.shape)} does not fit weight {tuple(weight.shape)}")
     _lib.ensure_device(x.device)
     dtype = _compute_dtype(x)
-    for t in (weight, *(() if bias is None else (bias,))):
-        engine._activation_code(t.dtype, "weight and bias")
-    engine._activation_code(dtype, "the type a linear layer computes in")
+    types = engine.ACTIVATION_DTYPES
+    if dtype not in types or weight.dtype not in types or (bias is not None and bias.dtype not in types):
+        raise TypeError(f"linear computes in float32, bfloat16 or float16, with weight and bias of these types; got "
+                        f"{dtype}, {weight.dtype}, {None if bias is None else bias.dtype}")
     if packed is not None:
         if packed.device != x.device:
             raise ValueError(f"input on {x.device}, checkpoint on {packed.device}")

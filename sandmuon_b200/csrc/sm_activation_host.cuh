@@ -408,7 +408,8 @@ int sm_weight_gradient(const void* delta, int dtype, int64_t n_rows, int64_t d_o
   memset(&p, 0, sizeof(p));
   const int64_t plane_elems = n_rows * g.plane_ld;
   const uint8_t* base = static_cast<const uint8_t*>(delta);
-  int64_t stride = std::max(row_stride, round_up(d_out, 8)) * 2;
+  // a single row has no stride of its own
+  int64_t stride = 2 * (n_rows == 1 ? g.plane_ld : row_stride);
   if (!g.direct) {
     uint16_t* planes = static_cast<uint16_t*>(workspace);
     const dim3 block(32, 8);

@@ -453,6 +453,14 @@ def gelu_backward(delta: torch.Tensor, values: torch.Tensor, exponents: torch.Te
     return out
 
 
+def column_sums(rows: torch.Tensor) -> torch.Tensor:
+    """rows.float().sum(0) of a 2-D tensor: the bias gradient of a linear layer."""
+    sums = rows.new_zeros((2, rows.shape[1]), dtype=torch.float32)
+    total = sums[1]
+    accumulate_column_stats(rows, sums[0], total)
+    return total
+
+
 def weight_gradient(delta: torch.Tensor, values: torch.Tensor, exponents: torch.Tensor, d_in: int,
                     dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """delta^T x^ [d_out, d_in] of a 2-D cotangent of any strides and a

@@ -322,3 +322,70 @@ def test_gpt2_memory():
     del out
     packed, out = peak("int8")
     assert packed < 0.75 * plain
+
+
+# ------------------------------------------------------------------ edge cases
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_weight_gradient_of_one_row_of_a_wider_tensor(dtype):
+    """A single row keeps whatever row stride its tensor had."""
+    base = cotangent(4, 21, dtype)
+    packed = activations.pack(activation(1, 50, dtype))
+    for delta in (base[:1, :16], base[0, :16], base[:1]):
+        check_weight_gradient(activations.weight_gradient(delta, packed), delta.reshape(1, -1), packed)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements: the last rows are packed, unpacked, summed and
+    multiplied like a small tensor of their own."""
+    rows, cols, tail = 70000, 32768, 96
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device=DEV)
+    x[-tail:] = activation(tail, cols, torch.bfloat16)
+    last = x[-tail:].clone()
+    packed = activations.pack(x, stats=True)
+    small = activations.pack(last, stats=True)
+    assert torch.equal(packed.values[-tail:], small.values) and torch.equal(packed.exponents[-tail:], small.exponents)
+    assert float((packed.sums - small.sums).norm() / small.sums.norm()) < 1e-6
+    delta = torch.zeros(rows, 40, dtype=torch.bfloat16, device=DEV)
+    delta[-tail:] = cotangent(tail, 40, torch.bfloat16)
+    dw, want = activations.weight_gradient(delta, packed), activations.weight_gradient(delta[-tail:], small)
+    assert float((dw - want).norm() / want.norm()) < 2e-6
+    del delta
+    out = activations.unpack(packed)
+    assert torch.equal(out[-tail:], small.unpack()) and not out[:1000].any()
+    del out
+    y, py = activations.gelu(x, pack_output=True)
+    assert torch.equal(y[-tail:], activations.gelu(last)) and not y[:1000].any()
+    del x
+    dx = activations.gelu_backward(y, packed)
+    assert torch.equal(dx[-tail:], activations.gelu_backward(y[-tail:], small))
+
+
+def test_first_call_inside_a_capture():
+    """A process whose first operator call is captured: nothing the library
+    sets up on first use breaks the capture."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import torch
+from sandmuon_b200 import activations
+x = torch.randn(3000, 300, device="cuda").bfloat16()
+d = torch.randn(3000, 200, device="cuda").bfloat16()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    packed = activations.pack(x, stats=True)
+    dw = activations.weight_gradient(d, packed)
+    dw32 = activations.weight_gradient(d.float(), packed)
+    y, py = activations.gelu(x, pack_output=True, stats=True)
+    dx = activations.gelu_backward(y, packed)
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(dw, activations.weight_gradient(d, activations.pack(x)))
+assert torch.equal(dx, activations.gelu_backward(y, activations.pack(x)))
+print("ok")
+"""
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                         cwd=Path(__file__).resolve().parents[1])
+    assert out.returncode == 0 and out.stdout.strip().endswith("ok"), out.stderr[-2000:]
