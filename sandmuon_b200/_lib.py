@@ -6,6 +6,8 @@ device is not an sm_100 GPU, every entry point raises instead of falling back.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 from pathlib import Path
@@ -156,6 +158,31 @@ def load() -> ctypes.CDLL:
                 fn.argtypes = argtypes
             _lib = lib
     return _lib
+
+
+BINDING_PATH = Path(__file__).resolve().parent / "_activations.so"
+_binding = None
+
+
+def binding():
+    """The torch extension of the activation operators (csrc/activations_binding.cpp),
+    bound to the library; raises if it has not been built."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    load()
+    with _lib_lock:
+        if _binding is None:
+            if not BINDING_PATH.exists():
+                raise RuntimeError(
+                    f"sandmuon_b200: {BINDING_PATH.name} is not built; run `python -m sandmuon_b200.csrc.build` "
+                    "(there is no CPU fallback)")
+            loader = importlib.machinery.ExtensionFileLoader("_activations", str(BINDING_PATH))
+            module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_activations", loader))
+            loader.exec_module(module)
+            module.bind(str(LIB_PATH))
+            _binding = module
+    return _binding
 
 
 def last_error() -> str:

@@ -1,9 +1,11 @@
-"""Builds libsandmuon_b200.so for sm_100a with nvcc, in-tree.
+"""Builds libsandmuon_b200.so for sm_100a with nvcc, and the torch extension of
+the activation operators with g++, in-tree.
 
 Usage:  python -m sandmuon_b200.csrc.build   (or sandmuon_b200.csrc.build.build())
 
-The shared library lands next to the package (sandmuon_b200/libsandmuon_b200.so)
-so it travels with the source tree; nothing is installed into site-packages.
+The shared objects land in the package (sandmuon_b200/libsandmuon_b200.so,
+sandmuon_b200/_activations.so) so they travel with the source tree; nothing is
+installed into site-packages.
 """
 from __future__ import annotations
 
@@ -11,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 CSRC = Path(__file__).resolve().parent
@@ -22,6 +25,10 @@ SOURCES = [CSRC / "libsandmuon_b200.cu"]
 DEPENDS = SOURCES + [CSRC / "sm_common.cuh", CSRC / "sm_gemm.cuh", CSRC / "sm_kernels.cuh",
                      CSRC / "sm_activation.cuh", CSRC / "sm_wgrad.cuh", CSRC / "sm_activation_host.cuh",
                      ROOT / "include" / "sandmuon_b200.h"]
+
+BINDING_PATH = PACKAGE / "_activations.so"
+BINDING_SOURCE = CSRC / "activations_binding.cpp"
+BINDING_DEPENDS = [BINDING_SOURCE, ROOT / "include" / "sandmuon_b200.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -38,27 +45,58 @@ def nvcc_path() -> str:
     raise RuntimeError("nvcc not found: the sandmuon_b200 CUDA library cannot be built")
 
 
-def up_to_date() -> bool:
-    if not LIB_PATH.exists():
+def up_to_date(target: Path = LIB_PATH, depends: list[Path] = DEPENDS) -> bool:
+    if not target.exists():
         return False
-    built = LIB_PATH.stat().st_mtime
-    return all(dep.stat().st_mtime <= built for dep in DEPENDS)
+    built = target.stat().st_mtime
+    return all(dep.stat().st_mtime <= built for dep in depends)
+
+
+def binding_command(out: Path) -> list[str]:
+    """g++ command of the torch extension."""
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    # not $CXX: a toolchain that links its own libstdc++ statically gives an
+    # extension whose exceptions and streams do not mix with torch's
+    compiler = shutil.which("g++")
+    if compiler is None:
+        raise RuntimeError("g++ not found: the sandmuon_b200 torch extension cannot be built")
+    cuda = Path(nvcc_path()).resolve().parents[1]
+    lib = Path(torch.__file__).resolve().parent / "lib"
+    includes = [*include_paths(), str(cuda / "include"), sysconfig.get_paths()["include"], str(ROOT / "include")]
+    return [compiler, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            "-DTORCH_EXTENSION_NAME=_activations", "-DTORCH_API_INCLUDE_EXTENSION_H",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *(f"-I{path}" for path in includes), "-o", str(out), str(BINDING_SOURCE), f"-L{lib}",
+            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python"]
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compiles the library unless it is newer than every source file."""
-    if not force and up_to_date():
-        return LIB_PATH
-    tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd = [nvcc_path(), *NVCC_FLAGS, "-I", str(ROOT / "include"), "-o", str(tmp), *map(str, SOURCES)]
-    if verbose:
-        print(" ".join(cmd), file=sys.stderr)
-    result = subprocess.run(cmd, capture_output=True, text=True)
-    if result.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({result.returncode}):\n{result.stdout}\n{result.stderr}")
-    if verbose and (result.stdout or result.stderr):
-        print(result.stdout + result.stderr, file=sys.stderr)
-    os.replace(tmp, LIB_PATH)
+    """Compiles the library and the extension, each unless it is newer than
+    every file it is made from; returns the library's path."""
+    jobs = []
+    for target, depends, command in (
+            (LIB_PATH, DEPENDS,
+             lambda out: [nvcc_path(), *NVCC_FLAGS, "-I", str(ROOT / "include"), "-o", str(out), *map(str, SOURCES)]),
+            (BINDING_PATH, BINDING_DEPENDS, binding_command)):
+        if not force and up_to_date(target, depends):
+            continue
+        tmp = target.with_suffix(".so.tmp")
+        cmd = command(tmp)
+        if verbose:
+            print(" ".join(cmd), file=sys.stderr)
+        jobs.append((target, tmp, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    failed = []
+    for target, tmp, process in jobs:
+        output = process.communicate()[0]
+        if process.returncode != 0:
+            failed.append(f"building {target.name} failed ({process.returncode}):\n{output}")
+            continue
+        if verbose and output:
+            print(output, file=sys.stderr)
+        os.replace(tmp, target)
+    if failed:
+        raise RuntimeError("\n".join(failed))
     return LIB_PATH
 
 

@@ -331,151 +331,3 @@ def apply_bf16_delta_multi(pairs: list[tuple[torch.Tensor, torch.Tensor]], devic
     with torch.cuda.device(device):
         rc = _lib.load().sm_apply_bf16_delta_multi(arr, len(pairs), _stream(device))
     _lib.check(rc, "sm_apply_bf16_delta_multi")
-
-
-# ------------------------------------------------ 8-bit activation checkpoints
-
-ACTIVATION_GROUP = 32
-ACTIVATION_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_GELU_FORMS = {"none": _lib.SM_GELU_ERF, "tanh": _lib.SM_GELU_TANH}
-
-
-def activation_ld(cols: int) -> int:
-    """Bytes of one row of a checkpoint's int8 values."""
-    return -(-cols // 16) * 16
-
-
-def activation_lde(cols: int) -> int:
-    """Bytes of one row of a checkpoint's exponent codes."""
-    return -(-cols // 128) * 4
-
-
-def _activation_code(dtype: torch.dtype, what: str) -> int:
-    code = ACTIVATION_DTYPES.get(dtype)
-    if code is None:
-        raise TypeError(f"{what} must be float32, bfloat16 or float16; got {dtype}")
-    return code
-
-
-def _gelu_form(approximate: str) -> int:
-    form = _GELU_FORMS.get(approximate)
-    if form is None:
-        raise ValueError(f'approximate must be "none" or "tanh"; got {approximate!r}')
-    return form
-
-
-def _rows_2d(t: torch.Tensor, what: str) -> torch.Tensor:
-    if t.dim() != 2:
-        raise ValueError(f"{what} must be 2-D [rows, columns]; got {tuple(t.shape)}")
-    _lib.ensure_device(t.device)
-    return t
-
-
-def _new_checkpoint(like: torch.Tensor, rows: int, cols: int) -> tuple[torch.Tensor, torch.Tensor]:
-    """Uninitialised (values, exponents) of a [rows, cols] activation on `like`'s device."""
-    return (like.new_empty((rows, activation_ld(cols)), dtype=torch.int8),
-            like.new_empty((rows, activation_lde(cols)), dtype=torch.uint8))
-
-
-def _sums_buffers(like: torch.Tensor, rows: int, cols: int):
-    """(result [2, cols], workspace or None, its bytes); the workspace belongs
-    to one call, so captured graphs and streams never share it."""
-    nbytes = _lib.load().sm_activation_sums_workspace_bytes(rows, cols)
-    ws = like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    return like.new_empty((2, cols), dtype=torch.float32), ws, nbytes
-
-
-def pack_activations(rows: torch.Tensor, stats: bool = False):
-    """(values, exponents, sums | None) of a 2-D activation of any strides;
-    sums is float32 [2, cols]: column sums of x^2 and of x."""
-    code = _activation_code(_rows_2d(rows, "an activation").dtype, "an activation")
-    device = rows.device
-    n, c = rows.shape
-    with _on(device):
-        values, exponents = _new_checkpoint(rows, n, c)
-        sums, ws, nbytes = _sums_buffers(rows, n, c) if stats else (None, None, 0)
-        rc = _lib.load().sm_activation_pack(
-            rows.data_ptr(), code, n, c, rows.stride(0), rows.stride(1), values.data_ptr(), exponents.data_ptr(),
-            0 if sums is None else sums.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes,
-            _lib.stream_handle(device))
-    _lib.check(rc, "sm_activation_pack")
-    return values, exponents, sums
-
-
-def unpack_activations(values: torch.Tensor, exponents: torch.Tensor, cols: int, dtype: torch.dtype) -> torch.Tensor:
-    """[rows, cols] contiguous tensor of the values a checkpoint stands for."""
-    code = _activation_code(dtype, "the unpacked type")
-    device = values.device
-    _lib.ensure_device(device)
-    n = values.shape[0]
-    with _on(device):
-        out = values.new_empty((n, cols), dtype=dtype)
-        rc = _lib.load().sm_activation_unpack(values.data_ptr(), exponents.data_ptr(), n, cols, out.data_ptr(), code,
-                                              _lib.stream_handle(device))
-    _lib.check(rc, "sm_activation_unpack")
-    return out
-
-
-def gelu_forward(rows: torch.Tensor, approximate: str, keep_input: bool, pack_output: bool, stats: bool):
-    """(y, (values, exponents) | None of x, (values, exponents, sums | None) | None of y)."""
-    code = _activation_code(_rows_2d(rows, "an activation").dtype, "an activation")
-    form = _gelu_form(approximate)
-    device = rows.device
-    n, c = rows.shape
-    with _on(device):
-        y = rows.new_empty((n, c))
-        kept = _new_checkpoint(rows, n, c) if keep_input else None
-        packed = _new_checkpoint(rows, n, c) if pack_output else None
-        sums, ws, nbytes = _sums_buffers(rows, n, c) if pack_output and stats else (None, None, 0)
-        rc = _lib.load().sm_gelu_forward(
-            rows.data_ptr(), code, n, c, rows.stride(0), rows.stride(1), form, y.data_ptr(),
-            kept[0].data_ptr() if keep_input else 0, kept[1].data_ptr() if keep_input else 0,
-            packed[0].data_ptr() if pack_output else 0, packed[1].data_ptr() if pack_output else 0,
-            0 if sums is None else sums.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes,
-            _lib.stream_handle(device))
-    _lib.check(rc, "sm_gelu_forward")
-    return y, kept, (*packed, sums) if pack_output else None
-
-
-def gelu_backward(delta: torch.Tensor, values: torch.Tensor, exponents: torch.Tensor,
-                  approximate: str) -> torch.Tensor:
-    """delta * gelu'(x^) for a 2-D cotangent of any strides; contiguous, delta's type."""
-    code = _activation_code(_rows_2d(delta, "a cotangent").dtype, "a cotangent")
-    form = _gelu_form(approximate)
-    device = delta.device
-    n, c = delta.shape
-    with _on(device):
-        out = delta.new_empty((n, c))
-        rc = _lib.load().sm_gelu_backward(delta.data_ptr(), code, n, c, delta.stride(0), delta.stride(1),
-                                          values.data_ptr(), exponents.data_ptr(), form, out.data_ptr(),
-                                          _lib.stream_handle(device))
-    _lib.check(rc, "sm_gelu_backward")
-    return out
-
-
-def column_sums(rows: torch.Tensor) -> torch.Tensor:
-    """rows.float().sum(0) of a 2-D tensor: the bias gradient of a linear layer."""
-    sums = rows.new_zeros((2, rows.shape[1]), dtype=torch.float32)
-    total = sums[1]
-    accumulate_column_stats(rows, sums[0], total)
-    return total
-
-
-def weight_gradient(delta: torch.Tensor, values: torch.Tensor, exponents: torch.Tensor, d_in: int,
-                    dtype: torch.dtype = torch.float32) -> torch.Tensor:
-    """delta^T x^ [d_out, d_in] of a 2-D cotangent of any strides and a
-    checkpoint of as many rows."""
-    code = _activation_code(_rows_2d(delta, "a cotangent").dtype, "a cotangent")
-    out_code = _activation_code(dtype, "a weight gradient")
-    device = delta.device
-    n, d_out = delta.shape
-    lib = _lib.load()
-    with _on(device):
-        out = delta.new_empty((d_out, d_in), dtype=dtype)
-        args = (delta.data_ptr(), code, n, d_out, delta.stride(0), delta.stride(1))
-        nbytes = lib.sm_weight_gradient_workspace_bytes(*args, d_in)
-        ws = delta.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-        rc = lib.sm_weight_gradient(*args, values.data_ptr(), exponents.data_ptr(), d_in, out.data_ptr(), out_code,
-                                    0 if ws is None else ws.data_ptr(), nbytes, _lib.stream_handle(device))
-    _lib.check(rc, "sm_weight_gradient")
-    return out

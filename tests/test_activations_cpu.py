@@ -9,7 +9,7 @@ import torch
 from torch import nn
 
 from oracle import activation_oracle as orc
-from sandmuon_b200 import RankOneAWeightedPE, _lib, activations, engine
+from sandmuon_b200 import RankOneAWeightedPE, _lib, activations
 from sandmuon_b200.workloads import GPT2, gpt2_matrix_filter
 
 
@@ -22,7 +22,7 @@ def cpu_packed(rows=3, cols=40, dtype=torch.bfloat16, **change):
 
 def test_layout_sizes():
     for cols, ld, lde in ((1, 16, 4), (16, 16, 4), (17, 32, 4), (128, 128, 4), (129, 144, 8), (768, 768, 24)):
-        assert (engine.activation_ld(cols), engine.activation_lde(cols)) == (ld, lde)
+        assert (activations.values_ld(cols), activations.exponents_ld(cols)) == (ld, lde)
         values, codes, _ = orc.checkpoint(np.ones((2, cols)), "float32")
         assert values.shape == (2, ld) and codes.shape == (2, lde)
     assert cpu_packed(shape=(1, 3, 40)).nbytes == 3 * 52
@@ -67,7 +67,7 @@ def test_cpu_tensors_fail_loudly(built_library):
             call()
 
 
-def test_argument_checks():
+def test_argument_checks(built_library):
     x = torch.randn(3, 40)
     scalar = torch.tensor(1.0)
     with pytest.raises(ValueError):
@@ -89,7 +89,7 @@ def test_argument_checks():
     with pytest.raises(ValueError, match="bias"):
         activations.linear(x, torch.randn(5, 40), torch.randn(4))
     with pytest.raises(ValueError, match="approximate"):
-        engine._gelu_form("sigmoid")
+        activations._gelu_form("sigmoid")
     with pytest.raises(ValueError, match="checkpoints"):
         GPT2(layers=1, width=8, heads=2, vocab=16, context=4, checkpoints="int4")
 

@@ -389,3 +389,15 @@ print("ok")
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
                          cwd=Path(__file__).resolve().parents[1])
     assert out.returncode == 0 and out.stdout.strip().endswith("ok"), out.stderr[-2000:]
+
+
+def test_gradients_can_be_recorded_but_not_differentiated():
+    x = activation(40, 64, torch.float32).requires_grad_()
+    w = torch.randn(16, 64, device=DEV).requires_grad_()
+    for y, leaves in ((activations.linear(x, w).square().sum(), [x, w]), (activations.gelu(x).square().sum(), [x])):
+        plain = torch.autograd.grad(y, leaves, retain_graph=True)
+        recorded = torch.autograd.grad(y, leaves, create_graph=True)
+        for a, b in zip(plain, recorded):
+            assert torch.equal(a, b)
+        with pytest.raises(RuntimeError, match="differentiate"):
+            torch.autograd.grad(recorded[0].sum(), leaves[0])
