@@ -64,6 +64,36 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
+// Two FP32 values in one 64-bit register pair, for the packed instructions of
+// sm_100: these kernels are bound by instruction issue, and one packed
+// instruction does two elements' work with the same roundings.
+struct Pair {
+  uint64_t v;
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(float a, float b) {
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  }
+  __device__ __forceinline__ explicit Pair(float both) : Pair(both, both) {}
+  __device__ __forceinline__ void get(float& a, float& b) const {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+  }
+};
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
 // Eight consecutive elements as 16-byte words, and their FP32 values.
 template <typename T>
 struct Vec8 {
@@ -222,8 +252,14 @@ __device__ __forceinline__ void pack8(int8_t* values, uint8_t* codes, const Vec8
   float inv = code_inverse(code);
   if (code >= CodeRange<T>::kHigh) rare_group<T>(max_bits, code, inv, v);
   uint32_t b[8];
+  const Pair inv2(inv), magic(kRoundMagic);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) b[i] = quantise_bits(v[i], inv);
+  for (int i = 0; i < 8; i += 2) {
+    float lo, hi;
+    fma2(Pair(v[i], v[i + 1]), inv2, magic).get(lo, hi);
+    b[i] = __float_as_uint(lo);
+    b[i + 1] = __float_as_uint(hi);
+  }
   if (FULL || (ok && in_values))
     *reinterpret_cast<uint2*>(values) = make_uint2(bytes4(b[0], b[1], b[2], b[3]), bytes4(b[4], b[5], b[6], b[7]));
   if ((threadIdx.x & 3) == 0 && (FULL || (ok && in_codes)))
@@ -275,9 +311,10 @@ __device__ __forceinline__ void unpack8(uint2 w, uint32_t code, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(__byte_perm(u[i / 4], 0x4b000000u, 0x7650u | (i & 3)));
   if (code <= kFusedCodes) {
-    const float s = __uint_as_float(code << 23), bias = -kByteBias * s;
+    const float s = __uint_as_float(code << 23);
+    const Pair scale(s), bias(-kByteBias * s);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], s, bias);
+    for (int i = 0; i < 8; i += 2) fma2(Pair(v[i], v[i + 1]), scale, bias).get(v[i], v[i + 1]);
   } else {
     const float s = code_scale(code);
 #pragma unroll
@@ -328,12 +365,35 @@ __device__ __forceinline__ ActLane act_lane(const ActGeometry& g) {
   return a;
 }
 
+// A lane's running sums of its 8 columns' squares and values.
+struct ColumnSums {
+  Pair sq[4], su[4];
+  __device__ __forceinline__ ColumnSums() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sq[i] = su[i] = Pair(0.0f);
+  }
+  __device__ __forceinline__ void add(const float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const Pair x(v[2 * i], v[2 * i + 1]);
+      sq[i] = fma2(x, x, sq[i]);
+      su[i] = add2(su[i], x);
+    }
+  }
+};
+
 // Column sums of one CTA: per-lane FP32 sums over its rows, joined across the
 // CTA's row lanes in a fixed order (FP64) and written to slot blockIdx.y of
 // partials [splits, 2, cols] -- or, with one split, to the result [2, cols].
 template <bool VEC>
-__device__ __forceinline__ void write_column_sums(const ActGeometry& g, const ActLane& a, const float (&sq)[8],
-                                                  const float (&su)[8], float* out) {
+__device__ __forceinline__ void write_column_sums(const ActGeometry& g, const ActLane& a, const ColumnSums& s,
+                                                  float* out) {
+  float sq[8], su[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s.sq[i].get(sq[2 * i], sq[2 * i + 1]);
+    s.su[i].get(su[2 * i], su[2 * i + 1]);
+  }
   __shared__ float sh[2][kActThreads * 8];
   const int width = VEC ? 8 << g.log_lanes : 256;  // columns of this CTA's strip
 #pragma unroll
@@ -383,8 +443,7 @@ __global__ void __launch_bounds__(32 * kFinishLanes)
 // Rows in flight per lane, and CTAs resident on an SM: a launch is one wave of
 // them.
 constexpr int kActUnroll = 4;
-constexpr int kPackCtas = 4, kUnpackCtas = 4, kGeluForwardCtas = 4;
-__host__ __device__ constexpr int gelu_backward_ctas(int elem_bytes) { return elem_bytes == 2 ? 6 : 4; }
+constexpr int kPackCtas = 4, kUnpackCtas = 4, kGeluForwardCtas = 4, kGeluBackwardCtas = 4;
 // The residency asked of the compiler; the strided mapping, bound by its
 // element accesses, is left its registers.
 __host__ __device__ constexpr int resident(bool vec, int ctas) { return vec ? ctas : 2; }
@@ -428,18 +487,7 @@ __global__ void __launch_bounds__(kActThreads, resident(VEC, kPackCtas))
     k_activation_pack(const T* __restrict__ x, int64_t rs, int64_t cs, ActGeometry g, Checkpoint c,
                       float* __restrict__ sums) {
   const ActLane a = act_lane<VEC>(g);
-  float sq[8], su[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) sq[i] = su[i] = 0.0f;
-  auto add = [&](const float(&v)[8]) {
-    if constexpr (STATS) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        sq[i] = fmaf(v[i], v[i], sq[i]);
-        su[i] += v[i];
-      }
-    }
-  };
+  ColumnSums column;
   if constexpr (VEC) {
     constexpr int kUnroll = sizeof(T) == 2 ? kActUnroll : 2;
     const bool in_x = a.col0 < g.cols, in_values = a.col0 < c.ld, in_codes = a.col0 / kGroup < c.lde;
@@ -460,7 +508,7 @@ __global__ void __launch_bounds__(kActThreads, resident(VEC, kPackCtas))
         vec8_unpack(w[u], v);
         pack8<T, kFull>(pp.values.take(), pp.codes.take(), w[u], v, r0 + u * a.row_lanes + a.row_lane < a.r_end,
                         in_values, in_codes);
-        add(v);
+        if (STATS) column.add(v);
       }
     });
   } else {
@@ -468,10 +516,10 @@ __global__ void __launch_bounds__(kActThreads, resident(VEC, kPackCtas))
       float v[8];
       load_strided(x, r, rs, cs, a.col0, g.cols, r < a.r_end, v);
       pack_strided<T>(c, r, r < a.r_end, a.col0, a.lane, v);
-      add(v);
+      if (STATS) column.add(v);
     }
   }
-  if (STATS) write_column_sums<VEC>(g, a, sq, su, sums);
+  if (STATS) write_column_sums<VEC>(g, a, column, sums);
   grid_dep_launch();
 }
 
@@ -546,52 +594,80 @@ constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 constexpr float kSqrt2OverPi = 0.79788456080286536f;
 constexpr float kGeluCubic = 0.044715f;
 
-// Phi(-|x|) / exp(-x^2 / 2), and exp(-x^2 / 2)
-__device__ __forceinline__ float normal_tail(float x, float& density) {
-  const float u = rcp_approx(fmaf(fabsf(x), 0.35f, 1.0f));
-  density = ex2_approx(x * (x * (-0.5f * kLog2E)));
-  float g = -0.029157886f;
-  g = fmaf(g, u, 0.14403091f);
-  g = fmaf(g, u, -0.25583899f);
-  g = fmaf(g, u, 0.15931970f);
-  g = fmaf(g, u, -0.023212353f);
-  g = fmaf(g, u, 0.10555250f);
-  g = fmaf(g, u, 0.11982129f);
-  g = fmaf(g, u, 0.13986352f);
-  g = fmaf(g, u, 0.13962130f);
-  return g * u;
+// For two elements: t = Phi(-|x|) / exp(-x^2 / 2) and d = exp(-x^2 / 2).
+__device__ __forceinline__ void normal_tail(float x0, float x1, Pair& t, Pair& d) {
+  const Pair x(x0, x1);
+  const Pair u(rcp_approx(fmaf(fabsf(x0), 0.35f, 1.0f)), rcp_approx(fmaf(fabsf(x1), 0.35f, 1.0f)));
+  float a0, a1;
+  mul2(x, mul2(x, Pair(-0.5f * kLog2E))).get(a0, a1);
+  d = Pair(ex2_approx(a0), ex2_approx(a1));
+  Pair g = fma2(Pair(-0.029157886f), u, Pair(0.14403091f));
+  g = fma2(g, u, Pair(-0.25583899f));
+  g = fma2(g, u, Pair(0.15931970f));
+  g = fma2(g, u, Pair(-0.023212353f));
+  g = fma2(g, u, Pair(0.10555250f));
+  g = fma2(g, u, Pair(0.11982129f));
+  g = fma2(g, u, Pair(0.13986352f));
+  g = fma2(g, u, Pair(0.13962130f));
+  t = mul2(g, u);
 }
 
 // The logistic function of 2 sqrt(2/pi) (x + 0.044715 x^3): the tanh form is
 // 0.5 (1 + tanh z) = 1 / (1 + exp(-2 z)).
-__device__ __forceinline__ float tanh_gate(float x, float x2) {
-  const float z = x * fmaf(x2, -2.0f * kLog2E * kSqrt2OverPi * kGeluCubic, -2.0f * kLog2E * kSqrt2OverPi);
-  return rcp_approx(1.0f + ex2_approx(z));
+__device__ __forceinline__ Pair tanh_gate(Pair x, Pair x2) {
+  constexpr float kScale = -2.0f * kLog2E * kSqrt2OverPi;
+  float z0, z1;
+  mul2(x, fma2(x2, Pair(kScale * kGeluCubic), Pair(kScale))).get(z0, z1);
+  return Pair(rcp_approx(1.0f + ex2_approx(z0)), rcp_approx(1.0f + ex2_approx(z1)));
 }
 
-// x = +inf gives inf and -inf gives NaN, as x * Phi(x) does in floating point.
+// v <- gelu(v).  +inf gives inf and -inf gives NaN, as x * Phi(x) does in
+// floating point.
 template <bool TANH>
-__device__ __forceinline__ float gelu_value(float x) {
-  if (TANH) return x * tanh_gate(x, x * x);
-  float density;
-  const float t = normal_tail(x, density);
-  return fmaf(-fabsf(fminf(x, 40.0f)), density * t, fmaxf(x, 0.0f));
-}
-
-template <bool TANH>
-__device__ __forceinline__ float gelu_slope(float x) {
-  if (TANH) {
-    // beyond |x| = 30 the slope is 0 or 1; the clamp (which lets NaN through)
-    // keeps x^2 finite
-    x = x > 30.0f ? 30.0f : x < -30.0f ? -30.0f : x;
-    const float x2 = x * x, s = tanh_gate(x, x2);
-    return fmaf(s * (1.0f - s), x * fmaf(x2, 6.0f * kSqrt2OverPi * kGeluCubic, 2.0f * kSqrt2OverPi), s);
+__device__ __forceinline__ void gelu_values(float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    if (TANH) {
+      const Pair x(v[i], v[i + 1]);
+      mul2(x, tanh_gate(x, mul2(x, x))).get(v[i], v[i + 1]);
+    } else {
+      Pair t, d;
+      normal_tail(v[i], v[i + 1], t, d);
+      float h0, h1;
+      mul2(d, t).get(h0, h1);
+      v[i] = fmaf(-fabsf(fminf(v[i], 40.0f)), h0, fmaxf(v[i], 0.0f));
+      v[i + 1] = fmaf(-fabsf(fminf(v[i + 1], 40.0f)), h1, fmaxf(v[i + 1], 0.0f));
+    }
   }
-  // Phi(x) + x phi(x) = [x >= 0] + exp(-x^2 / 2) (x / sqrt(2 pi) - sign(x) t),
-  // both by x's sign bit
-  float density;
-  const float t = normal_tail(x, density);
-  return fmaf(density, fmaf(x, kInvSqrt2Pi, -copysignf(t, x)), __float_as_int(x) >= 0 ? 1.0f : 0.0f);
+}
+
+// v <- d * gelu'(v)
+template <bool TANH>
+__device__ __forceinline__ void gelu_gradients(float (&v)[8], const float (&d)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    Pair slope;
+    if (TANH) {
+      // beyond |x| = 30 the slope is 0 or 1; the clamp (which lets NaN through)
+      // keeps x^2 finite
+      const float x0 = v[i] > 30.0f ? 30.0f : v[i] < -30.0f ? -30.0f : v[i];
+      const float x1 = v[i + 1] > 30.0f ? 30.0f : v[i + 1] < -30.0f ? -30.0f : v[i + 1];
+      const Pair x(x0, x1), x2 = mul2(x, x), s = tanh_gate(x, x2);
+      const Pair inner = mul2(x, fma2(x2, Pair(6.0f * kSqrt2OverPi * kGeluCubic), Pair(2.0f * kSqrt2OverPi)));
+      slope = fma2(mul2(s, fma2(s, Pair(-1.0f), Pair(1.0f))), inner, s);
+    } else {
+      // Phi(x) + x phi(x) = [x >= 0] + exp(-x^2 / 2) (x / sqrt(2 pi) - sign(x) t),
+      // both by x's sign bit
+      Pair t, density;
+      normal_tail(v[i], v[i + 1], t, density);
+      float t0, t1;
+      t.get(t0, t1);
+      const Pair minus(-copysignf(t0, v[i]), -copysignf(t1, v[i + 1]));
+      const Pair step(__float_as_int(v[i]) >= 0 ? 1.0f : 0.0f, __float_as_int(v[i + 1]) >= 0 ? 1.0f : 0.0f);
+      slope = fma2(density, fma2(Pair(v[i], v[i + 1]), Pair(kInvSqrt2Pi), minus), step);
+    }
+    mul2(Pair(d[i], d[i + 1]), slope).get(v[i], v[i + 1]);
+  }
 }
 
 // y = gelu(x); packs x into `in` (PACK_IN) and the rounded y into `out` with
@@ -601,18 +677,7 @@ __global__ void __launch_bounds__(kActThreads, resident(VEC, kGeluForwardCtas))
     k_gelu_forward(const T* __restrict__ x, int64_t rs, int64_t cs, ActGeometry g, T* __restrict__ y, Checkpoint in,
                    Checkpoint out, float* __restrict__ sums) {
   const ActLane a = act_lane<VEC>(g);
-  float sq[8], su[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) sq[i] = su[i] = 0.0f;
-  auto add = [&](const float(&v)[8]) {
-    if constexpr (PACK_OUT) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        sq[i] = fmaf(v[i], v[i], sq[i]);
-        su[i] += v[i];
-      }
-    }
-  };
+  ColumnSums column;
   if constexpr (VEC) {
     constexpr int kUnroll = 2;
     const bool in_x = a.col0 < g.cols, in_values = a.col0 < in.ld, in_codes = a.col0 / kGroup < in.lde;
@@ -634,15 +699,14 @@ __global__ void __launch_bounds__(kActThreads, resident(VEC, kGeluForwardCtas))
         float v[8];
         vec8_unpack(w[u], v);
         if (PACK_IN) pack8<T, kFull>(ip.values.take(), ip.codes.take(), w[u], v, ok, in_values, in_codes);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = gelu_value<TANH>(v[i]);
+        gelu_values<TANH>(v);
         vec8_pack(v, w[u]);
         T* at = yp.take();
         if (kFull || (in_x && ok)) vec8_store(at, w[u]);
         if (PACK_OUT) {
           vec8_unpack(w[u], v);
           pack8<T, kFull>(op.values.take(), op.codes.take(), w[u], v, ok, in_values, in_codes);
-          add(v);
+          column.add(v);
         }
       }
     });
@@ -652,27 +716,28 @@ __global__ void __launch_bounds__(kActThreads, resident(VEC, kGeluForwardCtas))
       float v[8];
       load_strided(x, r, rs, cs, a.col0, g.cols, ok, v);
       if (PACK_IN) pack_strided<T>(in, r, ok, a.col0, a.lane, v);
+      gelu_values<TANH>(v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = to_f32(from_f32<T>(gelu_value<TANH>(v[i])));
+      for (int i = 0; i < 8; ++i) v[i] = to_f32(from_f32<T>(v[i]));
       store_strided(y, r, a.col0, g.cols, ok, v);
       if (PACK_OUT) {
         pack_strided<T>(out, r, ok, a.col0, a.lane, v);
-        add(v);
+        column.add(v);
       }
     }
   }
-  if (PACK_OUT && sums != nullptr) write_column_sums<VEC>(g, a, sq, su, sums);
+  if (PACK_OUT && sums != nullptr) write_column_sums<VEC>(g, a, column, sums);
   grid_dep_launch();
 }
 
 // dx = delta * gelu'(x^)
 template <typename T, bool VEC, bool TANH>
-__global__ void __launch_bounds__(kActThreads, resident(VEC, gelu_backward_ctas(sizeof(T))))
+__global__ void __launch_bounds__(kActThreads, resident(VEC, kGeluBackwardCtas))
     k_gelu_backward(const T* __restrict__ delta, int64_t rs, int64_t cs, ActGeometry g, Checkpoint c,
                     T* __restrict__ dx) {
   const ActLane a = act_lane<VEC>(g);
   if constexpr (VEC) {
-    constexpr int kUnroll = 2;
+    constexpr int kUnroll = sizeof(T) == 2 ? kActUnroll : 2;
     const bool in_x = a.col0 < g.cols;
     RowPointer<const T> dp(delta, a.r_begin + a.row_lane, rs, a.col0, a.row_lanes);
     RowPointer<T> op(dx, a.r_begin + a.row_lane, g.cols, a.col0, a.row_lanes);
@@ -700,8 +765,7 @@ __global__ void __launch_bounds__(kActThreads, resident(VEC, gelu_backward_ctas(
           float v[8], dv[8];
           unpack8(w[u], code[u], v);
           vec8_unpack(d[u], dv);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = dv[i] * gelu_slope<TANH>(v[i]);
+          gelu_gradients<TANH>(v, dv);
           vec8_pack(v, d[u]);
           vec8_store(at, d[u]);
         }
@@ -712,8 +776,7 @@ __global__ void __launch_bounds__(kActThreads, resident(VEC, gelu_backward_ctas(
       float v[8], d[8];
       unpack_strided(c, r, true, a.col0, g.cols, v);
       load_strided(delta, r, rs, cs, a.col0, g.cols, true, d);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = d[i] * gelu_slope<TANH>(v[i]);
+      gelu_gradients<TANH>(v, d);
       store_strided(dx, r, a.col0, g.cols, true, v);
     }
   }

@@ -361,7 +361,7 @@ int sm_gelu_backward(const void* delta, int dtype, int64_t n_rows, int64_t n_col
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool vec = vec8_rows(delta, dtype, n_rows, n_cols, row_stride, col_stride) &&
                    vec8_rows(dx, dtype, n_rows, n_cols, n_cols, 1);
-  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms, gelu_backward_ctas(elem_size(dtype)));
+  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms, kGeluBackwardCtas);
   const Checkpoint c = act_checkpoint(values, exponents, n_cols);
   const bool th = form == SM_GELU_TANH;
   if (dtype == SM_DTYPE_F32)
