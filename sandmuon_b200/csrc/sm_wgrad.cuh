@@ -14,7 +14,7 @@
 // (cta_group::2): each CTA stages 128 delta columns and 128 x^ columns.
 //   warp 0        delta producer: TMA loads (128-byte swizzle), counted on the
 //                 leader's barrier
-//   warp 1        MMA issuer (the leader's thread, for both CTAs)
+//   warp 1        MMA issuer (the leader's warp, for both CTAs)
 //   warp 2        raw producer: TMA loads of the int8 tiles
 //   warp 3        code producer: 4-byte asynchronous copies of their exponents
 //   warps 4..11   epilogue: TMEM -> registers -> global
@@ -50,8 +50,9 @@ constexpr int kWgConvWarps = 16;
 constexpr int kWgConvGroups = 4;
 constexpr int kWgEpiWarps = 8;
 constexpr int kWgChain = 128;  // MMA steps summed by the tensor core alone
-// Warps 0..3 issue loads and MMAs; then come the epilogue and the converters, each whole groups of four warps that trade registers
-// (setmaxnreg): the launch's 28 warps of 72 cover 4 of 40, 8 of 104 and 16 of 64.
+// Warps 0..3 issue loads and MMAs; then come the epilogue and the converters,
+// each whole groups of four warps that trade registers (setmaxnreg): the
+// launch's 28 warps of 72 registers cover 4 of 40, 8 of 104 and 16 of 64.
 constexpr int kWgEpiWarp0 = 4, kWgConvWarp0 = kWgEpiWarp0 + kWgEpiWarps;
 constexpr int kWgThreads = 32 * (kWgConvWarp0 + kWgConvWarps);
 constexpr int kWgLaunchRegs = 72, kWgIssueRegs = 40, kWgEpiRegs = 104, kWgConvRegs = 64;
@@ -560,7 +561,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
     // ---------------------------------------------------------- MMA issuer
     // The whole warp walks the loop, so that descriptors and barriers stay in
     // uniform registers; one elected lane issues.  (One lane alone in a
-    // divergent branch took 95 clocks an MMA, longer than its 128 allow for.)
+    // divergent branch took 95 clocks to issue an MMA that runs for 128.)
     if (rank == 0) {
       const bool elected = elect_one();
       WgRing<S::kAStages> ra;
@@ -630,8 +631,8 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
   } else if (warp >= kWgEpiWarp0 && warp < kWgConvWarp0) {
     // ------------------------------------------------------------ epilogue
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWgEpiRegs));
-    const int quarter = warp & 3;           // TMEM lanes this warp may access
-    const int half = (warp - kWgEpiWarp0) >> 2;       // its 128 of the tile's 256 columns
+    const int quarter = warp & 3;                // TMEM lanes this warp may access
+    const int half = (warp - kWgEpiWarp0) >> 2;  // its 128 of the tile's 256 columns
     const uint32_t tempty0 = mapa_shared(bar_tempty(0), 0);
     float* stg = reinterpret_cast<float*>(smem + S::kOffStaging) + (warp - kWgEpiWarp0) * 32 * 9;
     auto release = [&](int acc) {
@@ -793,6 +794,10 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
     }
   }
 
+  // After a wait that ran out, copies may still be in flight into this CTA's
+  // shared memory, which has to outlive them: leave 100 us later.
+  if (*abort_flag != 0)
+    for (int i = 0; i < 100; ++i) __nanosleep(1000);
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();

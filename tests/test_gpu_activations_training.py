@@ -401,3 +401,25 @@ def test_gradients_can_be_recorded_but_not_differentiated():
             assert torch.equal(a, b)
         with pytest.raises(RuntimeError, match="differentiate"):
             torch.autograd.grad(recorded[0].sum(), leaves[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_weight_gradient_of_the_largest_and_smallest_values(dtype):
+    """Checkpoints at both ends of their exponents, next to ordinary ones."""
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn(300, 160, generator=g).double()
+    top = 6e4 if dtype == torch.float16 else 3e38
+    x[:, :32] *= top / x[:, :32].abs().max()
+    x[:, 32:64] *= 5000 if dtype == torch.float16 else 1e30
+    x[:, 64:96] *= torch.finfo(dtype).smallest_normal * 64
+    x[7, 96:128] = 0
+    x = x.to(dtype).to(DEV)
+    delta = (torch.randn(300, 70, generator=g) * (1e-3 if dtype == torch.float16 else 1e-6)).to(dtype).to(DEV)
+    packed = activations.pack(x)
+    got = activations.weight_gradient(delta, packed)
+    d, hat = delta.double(), packed.unpack(torch.float32).double()
+    want, size = d.t() @ hat, d.abs().t() @ hat.abs()
+    # a subnormal product or plane of the cotangent is off by at most 2^-133 a term
+    assert ((got.double() - want).abs() <= 400 * 3 * 2.0 ** -23 * size + 900 * 2.0 ** -133 * (1 + hat.abs().max())).all()
+    assert float(((got.double() - want) / size.clamp_min(1e-300))[:, :64].abs().max()) < 1e-5
+    assert float(((got.double() - want) / size.clamp_min(1e-300))[:, 96:].abs().max()) < 1e-5
