@@ -763,8 +763,6 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
         w[t] = lds128(slot_raw(rr.slot) + in_off + t * (kTaskRows * 128));
         code[t] = lds8(slot_codes(rr.slot) + code_off + t * (kTaskRows * 4));
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_rempty(rr.slot));
       if (i >= S::kBStages) {
         ok = mbar_wait(bar_done(rd.slot), rd.phase, abort_flag, kStatusTimeoutWgradConvert);
         if (!__all_sync(0xffffffffu, ok)) break;
@@ -783,6 +781,12 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
         sts128(slot_b(rb.slot) + off0 + t * (kTaskRows * 128), a0.x, a0.y, a1.x, a1.y);
         sts128(slot_b(rb.slot) + off1 + t * (kTaskRows * 128), b0.x, b0.y, b1.x, b1.y);
       }
+      // Every value read from the raw slot has been used, so the loads are done
+      // and the slot is free.  (Released right after the loads were issued, the
+      // slot's next codes could overtake a delayed load: about one k-block in a
+      // million came out with some tokens at a wrong scale.)
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_rempty(rr.slot));
       // The MMA that these arrivals admit reads this tile through this CTA's
       // own async proxy, to which the fence has made it visible; no data is
       // handed to the peer, so the arrival carries no cluster-scope release

@@ -423,3 +423,26 @@ def test_weight_gradient_of_the_largest_and_smallest_values(dtype):
     assert ((got.double() - want).abs() <= 400 * 3 * 2.0 ** -23 * size + 900 * 2.0 ** -133 * (1 + hat.abs().max())).all()
     assert float(((got.double() - want) / size.clamp_min(1e-300))[:, :64].abs().max()) < 1e-5
     assert float(((got.double() - want) / size.clamp_min(1e-300))[:, 96:].abs().max()) < 1e-5
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_weight_gradient_repeats_bit_for_bit_under_load(dtype):
+    """Back-to-back calls over two sets of inputs that fill every SM: the sums
+    run in a fixed order, so each call returns the same bits.  (A k-block that
+    is read before it is complete, or after its slot was given back, shows
+    here; it took about one k-block in a million.)"""
+    rows, d_in, d_out = 16384, 2048, 4096 if dtype == torch.float32 else 8192
+    sets = []
+    for seed in (1, 2):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        x = torch.randn(rows, d_in, generator=g, device=DEV) * torch.exp(torch.randn(rows, 1, generator=g, device=DEV))
+        delta = torch.randn(rows, d_out, generator=g, device=DEV) * 0.1
+        packed, delta = activations.pack(x.to(dtype)), delta.to(dtype)
+        sets.append((delta, packed, activations.weight_gradient(delta, packed)))
+    del x
+    wrong = torch.zeros((), dtype=torch.int64, device=DEV)
+    for _ in range(60):
+        for delta, packed, want in sets:
+            wrong += (activations.weight_gradient(delta, packed) != want).sum()
+    assert int(wrong) == 0
+    assert _lib.device_status(DEV) == 0
