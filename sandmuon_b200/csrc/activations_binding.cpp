@@ -217,24 +217,28 @@ Tensor gelu_backward(const Tensor& delta, const Tensor& values, const Tensor& co
   return as_shape(gelu_backward_rows(flat(delta.detach(), "a cotangent"), values, codes, form), delta.sizes());
 }
 
-// Gradients of a backward pass that itself is recorded (create_graph): usable,
-// and an error once something differentiates through them.
-variable_list once(variable_list grads, bool recorded) {
-  if (!recorded) return grads;
-  variable_list aliases, out;
-  for (const Tensor& g : grads) {
-    if (!g.defined()) continue;
-    Tensor a = g.detach();
+// Gradients of a backward pass that itself is recorded (create_graph).  Those
+// that depend on something with a gradient -- the cotangent, or a tensor of the
+// forward pass -- are usable, and an error once something differentiates
+// through them; the others are constants.
+variable_list once(variable_list grads, const std::vector<bool>& depends) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list aliases;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    if (!grads[i].defined() || !depends[i]) continue;
+    Tensor a = grads[i].detach();
     a.set_requires_grad(true);
     aliases.push_back(a);
   }
+  if (aliases.empty()) return grads;
   torch::autograd::DelayedError error(
       "trying to differentiate twice a function of sandmuon_b200.activations, which can be differentiated once",
       static_cast<int64_t>(aliases.size()));
   const variable_list marked = error.apply(std::move(aliases));
   size_t next = 0;
-  for (const Tensor& g : grads) out.push_back(g.defined() ? marked[next++] : Tensor());
-  return out;
+  for (size_t i = 0; i < grads.size(); ++i)
+    if (grads[i].defined() && depends[i]) grads[i] = marked[next++];
+  return grads;
 }
 
 struct Linear : torch::autograd::Function<Linear> {
@@ -246,25 +250,29 @@ struct Linear : torch::autograd::Function<Linear> {
     ctx->saved_data["weight"] = static_cast<int64_t>(weight.scalar_type());
     ctx->saved_data["bias"] = static_cast<int64_t>(bias ? bias->scalar_type() : at::kFloat);
     ctx->saved_data["shape"] = x.sizes();
+    ctx->saved_data["x_grad"] = x.requires_grad();
     optional<Tensor> b;
     if (bias) b = bias->to(dtype);
     return at::linear(x, cast, b);
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const bool recorded = at::GradMode::is_enabled() && grads[0].requires_grad();
-    const at::NoGradGuard no_grad;
-    const variable_list saved = ctx->get_saved_variables();
-    const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
-    const Tensor rows = flat(grads[0], "a cotangent");
+    const bool delta_grad = grads[0].requires_grad();
     variable_list out(5);
-    if (ctx->needs_input_grad(0)) out[0] = as_shape(at::mm(rows, saved[0]), shape);
-    if (ctx->needs_input_grad(1))
-      out[1] = weight_gradient_rows(rows, saved[1], saved[2], shape.back(),
-                                    static_cast<at::ScalarType>(ctx->saved_data["weight"].toInt()));
-    if (ctx->needs_input_grad(2))
-      out[2] = column_sums(rows).to(static_cast<at::ScalarType>(ctx->saved_data["bias"].toInt()));
-    return once(std::move(out), recorded);
+    {
+      const at::NoGradGuard no_grad;
+      const variable_list saved = ctx->get_saved_variables();
+      const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+      const Tensor rows = flat(grads[0], "a cotangent");
+      if (ctx->needs_input_grad(0)) out[0] = as_shape(at::mm(rows, saved[0]), shape);
+      if (ctx->needs_input_grad(1))
+        out[1] = weight_gradient_rows(rows, saved[1], saved[2], shape.back(),
+                                      static_cast<at::ScalarType>(ctx->saved_data["weight"].toInt()));
+      if (ctx->needs_input_grad(2))
+        out[2] = column_sums(rows).to(static_cast<at::ScalarType>(ctx->saved_data["bias"].toInt()));
+    }
+    // delta W (W has a gradient, or this node would not be), delta^T x^, sum delta
+    return once(std::move(out), {true, delta_grad || ctx->saved_data["x_grad"].toBool(), delta_grad, false, false});
   }
 };
 
@@ -324,12 +332,15 @@ struct Gelu : torch::autograd::Function<Gelu> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const bool recorded = at::GradMode::is_enabled() && grads[0].requires_grad();
-    const at::NoGradGuard no_grad;
-    const variable_list saved = ctx->get_saved_variables();
-    const Tensor dx = gelu_backward_rows(flat(grads[0], "a cotangent"), saved[0], saved[1],
-                                         ctx->saved_data["form"].toInt());
-    return once({as_shape(dx, grads[0].sizes()), Tensor(), Tensor(), Tensor()}, recorded);
+    variable_list out(4);
+    {
+      const at::NoGradGuard no_grad;
+      const variable_list saved = ctx->get_saved_variables();
+      const Tensor dx = gelu_backward_rows(flat(grads[0], "a cotangent"), saved[0], saved[1],
+                                           ctx->saved_data["form"].toInt());
+      out[0] = as_shape(dx, grads[0].sizes());
+    }
+    return once(std::move(out), {true, false, false, false});  // x has a gradient, or this node would not be
   }
 };
 

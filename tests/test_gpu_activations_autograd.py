@@ -1,0 +1,82 @@
+"""The 8-bit checkpoint operators inside autograd: second and forward
+derivatives, tracing, in-place changes of outputs, memory of a backward pass.
+
+An operator that cannot give what is asked of it raises; it never returns a
+constant in its place."""
+import pytest
+import torch
+
+from sandmuon_b200 import activations
+from test_gpu_activations import DTYPES, activation, cotangent
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+
+
+def weight(d_out, d_in, seed=0):
+    g = torch.Generator().manual_seed(seed + 7 * d_out + d_in)
+    return (torch.randn(d_out, d_in, generator=g) * .05).to(DEV).requires_grad_()
+
+
+# --------------------------------------------------------- second derivatives
+
+def test_a_penalty_on_the_input_gradient_of_a_linear_layer_raises():
+    """d(sum y)/dx = 1^T W depends on the weight although the cotangent is a
+    constant."""
+    x, w = activation(40, 64, torch.float32).requires_grad_(), weight(16, 64)
+    b = torch.zeros(16, device=DEV, requires_grad=True)
+    for bias in (None, b):
+        y = activations.linear(x, w, bias)
+        g, = torch.autograd.grad(y.sum(), x, create_graph=True)
+        assert torch.equal(g, torch.ones(40, 16, device=DEV) @ w.detach())
+        with pytest.raises(RuntimeError, match="differentiate"):
+            (y.sum() + g.square().sum()).backward()
+
+
+def test_a_penalty_on_the_weight_gradient_raises_where_the_input_has_a_gradient():
+    """d(sum y)/dW = 1^T x depends on x: an error for an x with a gradient, a
+    constant for data."""
+    w = weight(16, 64)
+    x = activation(40, 64, torch.float32)
+    for leaf in (x.clone().requires_grad_(), x):
+        y = activations.linear(leaf, w)
+        g, = torch.autograd.grad(y.sum(), w, create_graph=True)
+        assert torch.equal(g, activations.weight_gradient(torch.ones(40, 16, device=DEV), activations.pack(x)))
+        if leaf.requires_grad:
+            with pytest.raises(RuntimeError, match="differentiate"):
+                g.square().sum().backward()
+        else:
+            assert not g.requires_grad
+
+
+def test_a_recorded_bias_gradient_of_a_constant_cotangent_is_a_constant():
+    x, w = activation(40, 64, torch.float32).requires_grad_(), weight(16, 64)
+    b = torch.zeros(16, device=DEV, requires_grad=True)
+    g, = torch.autograd.grad(activations.linear(x, w, b).sum(), b, create_graph=True)
+    assert torch.equal(g, torch.full((16,), 40.0, device=DEV)) and not g.requires_grad
+    loss = activations.linear(x, w, b).square().sum()  # a cotangent that depends on the bias
+    g, = torch.autograd.grad(loss, b, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate"):
+        g.sum().backward()
+
+
+@pytest.mark.parametrize("approximate", ["none", "tanh"])
+def test_a_penalty_on_the_gradient_of_gelu_raises(approximate):
+    x = activation(40, 64, torch.float32).requires_grad_()
+    for pack_output in (False, True):
+        y = activations.gelu(x, approximate=approximate, pack_output=pack_output)
+        y = y[0] if pack_output else y
+        g, = torch.autograd.grad(y.sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate"):
+            (y.sum() + g.square().sum()).backward()
+
+
+def test_recorded_gradients_are_the_plain_ones():
+    x, w = activation(40, 64, torch.float32).requires_grad_(), weight(16, 64)
+    b = torch.zeros(16, device=DEV, requires_grad=True)
+    delta = cotangent(40, 16, torch.float32)
+    y = activations.linear(x, w, b)
+    plain = torch.autograd.grad(y, [x, w, b], delta, retain_graph=True)
+    recorded = torch.autograd.grad(y, [x, w, b], delta, create_graph=True)
+    for p, r in zip(plain, recorded):
+        assert torch.equal(p, r) and not p.requires_grad
