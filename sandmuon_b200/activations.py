@@ -133,7 +133,9 @@ def weight_gradient(delta: torch.Tensor, packed: PackedActivation, *,
                     dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """dW [d_out, d_in] = delta^T x^ of a linear layer with output cotangent
     delta [..., d_out] and packed input [..., d_in], summed in FP32.  A float16
-    cotangent needs a checkpoint packed from float16 values."""
+    cotangent needs a checkpoint packed from float16 values.  Not
+    differentiable: with a delta that takes a gradient the result raises once
+    something differentiates through it."""
     cols = packed.shape[-1]
     _fits(packed, delta, (*delta.shape[:-1], cols), "the rows of a cotangent with")
     if delta.dtype == torch.float16 and packed.dtype != torch.float16:
@@ -195,6 +197,7 @@ def gelu(x: torch.Tensor, *, approximate: str = "none", pack_output: bool = Fals
 
 def gelu_backward(delta: torch.Tensor, packed: PackedActivation, *, approximate: str = "none") -> torch.Tensor:
     """delta * gelu'(x^) for the checkpoint of GELU's input, in delta's type:
-    what `gelu` runs in its backward pass."""
+    what `gelu` runs in its backward pass.  Not differentiable, as
+    `weight_gradient`."""
     _fits(packed, delta, delta.shape, "a cotangent")
     return _lib.binding().gelu_backward(delta, packed.values, packed.exponents, _gelu_form(approximate))

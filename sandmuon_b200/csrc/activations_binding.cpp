@@ -109,6 +109,31 @@ struct Workspace {
 
 void* ptr(const optional<Tensor>& t) { return t ? t->data_ptr() : nullptr; }
 
+// Gradients that are computed while autograd records (a backward pass with
+// create_graph, or a call of a backward operator).  Those that depend on
+// something with a gradient -- the cotangent, or a tensor of the forward pass --
+// are usable, and an error once something differentiates through them; the
+// others are constants.
+variable_list once(variable_list grads, const std::vector<bool>& depends) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list aliases;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    if (!grads[i].defined() || !depends[i]) continue;
+    Tensor a = grads[i].detach();
+    a.set_requires_grad(true);
+    aliases.push_back(a);
+  }
+  if (aliases.empty()) return grads;
+  torch::autograd::DelayedError error(
+      "trying to differentiate twice a function of sandmuon_b200.activations, which can be differentiated once",
+      static_cast<int64_t>(aliases.size()));
+  const variable_list marked = error.apply(std::move(aliases));
+  size_t next = 0;
+  for (size_t i = 0; i < grads.size(); ++i)
+    if (grads[i].defined() && depends[i]) grads[i] = marked[next++];
+  return grads;
+}
+
 using Packed = std::tuple<Tensor, Tensor, optional<Tensor>>;
 
 Packed pack_rows(const Tensor& x, bool stats) {
@@ -158,7 +183,8 @@ Tensor weight_gradient_rows(const Tensor& delta, const Tensor& values, const Ten
 
 Tensor weight_gradient(const Tensor& delta, const Tensor& values, const Tensor& codes, int64_t d_in,
                        at::ScalarType dtype) {
-  return weight_gradient_rows(flat(delta.detach(), "a cotangent"), values, codes, d_in, dtype);
+  return once({weight_gradient_rows(flat(delta.detach(), "a cotangent"), values, codes, d_in, dtype)},
+              {delta.requires_grad()})[0];
 }
 
 // delta.float().sum(0): the column sums of the statistics kernels.
@@ -214,31 +240,8 @@ Tensor gelu_backward_rows(const Tensor& delta, const Tensor& values, const Tenso
 Tensor as_shape(const Tensor& t, at::IntArrayRef shape) { return t.sizes() == shape ? t : t.view(shape); }
 
 Tensor gelu_backward(const Tensor& delta, const Tensor& values, const Tensor& codes, int64_t form) {
-  return as_shape(gelu_backward_rows(flat(delta.detach(), "a cotangent"), values, codes, form), delta.sizes());
-}
-
-// Gradients of a backward pass that itself is recorded (create_graph).  Those
-// that depend on something with a gradient -- the cotangent, or a tensor of the
-// forward pass -- are usable, and an error once something differentiates
-// through them; the others are constants.
-variable_list once(variable_list grads, const std::vector<bool>& depends) {
-  if (!at::GradMode::is_enabled()) return grads;
-  variable_list aliases;
-  for (size_t i = 0; i < grads.size(); ++i) {
-    if (!grads[i].defined() || !depends[i]) continue;
-    Tensor a = grads[i].detach();
-    a.set_requires_grad(true);
-    aliases.push_back(a);
-  }
-  if (aliases.empty()) return grads;
-  torch::autograd::DelayedError error(
-      "trying to differentiate twice a function of sandmuon_b200.activations, which can be differentiated once",
-      static_cast<int64_t>(aliases.size()));
-  const variable_list marked = error.apply(std::move(aliases));
-  size_t next = 0;
-  for (size_t i = 0; i < grads.size(); ++i)
-    if (grads[i].defined() && depends[i]) grads[i] = marked[next++];
-  return grads;
+  return once({as_shape(gelu_backward_rows(flat(delta.detach(), "a cotangent"), values, codes, form), delta.sizes())},
+              {delta.requires_grad()})[0];
 }
 
 struct Linear : torch::autograd::Function<Linear> {

@@ -80,3 +80,18 @@ def test_recorded_gradients_are_the_plain_ones():
     recorded = torch.autograd.grad(y, [x, w, b], delta, create_graph=True)
     for p, r in zip(plain, recorded):
         assert torch.equal(p, r) and not p.requires_grad
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_operators_on_a_cotangent_with_a_gradient(dtype):
+    """Their results can be used, and raise once something differentiates
+    through them: they depend on the cotangent."""
+    delta = cotangent(40, 64, dtype)
+    packed = activations.pack(activation(40, 64, dtype))
+    for call in (activations.weight_gradient, activations.gelu_backward):
+        got = call(delta.clone().requires_grad_(), packed)
+        assert torch.equal(got, call(delta, packed))
+        with pytest.raises(RuntimeError, match="differentiate"):
+            got.float().sum().backward()
+        with torch.no_grad():
+            assert not call(delta.clone().requires_grad_(), packed).requires_grad
