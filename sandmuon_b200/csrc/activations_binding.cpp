@@ -73,6 +73,13 @@ void on_gpu(const Tensor& t) {
   TORCH_CHECK(t.is_cuda(), "sandmuon_b200 runs on CUDA (sm_100) tensors only; got a tensor on ", t.device());
 }
 
+// The operators have no rule for forward-mode derivatives; their kernels would
+// drop a tangent without a word.
+void no_tangent(const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(),
+                              "sandmuon_b200.activations has no forward-mode derivatives");
+}
+
 std::string text(const Tensor& t) {
   std::string s = "[";
   for (int64_t d = 0; d < t.dim(); ++d) s += (d ? ", " : "") + std::to_string(t.size(d));
@@ -183,6 +190,7 @@ Tensor weight_gradient_rows(const Tensor& delta, const Tensor& values, const Ten
 
 Tensor weight_gradient(const Tensor& delta, const Tensor& values, const Tensor& codes, int64_t d_in,
                        at::ScalarType dtype) {
+  no_tangent(delta);
   return once({weight_gradient_rows(flat(delta.detach(), "a cotangent"), values, codes, d_in, dtype)},
               {delta.requires_grad()})[0];
 }
@@ -240,6 +248,7 @@ Tensor gelu_backward_rows(const Tensor& delta, const Tensor& values, const Tenso
 Tensor as_shape(const Tensor& t, at::IntArrayRef shape) { return t.sizes() == shape ? t : t.view(shape); }
 
 Tensor gelu_backward(const Tensor& delta, const Tensor& values, const Tensor& codes, int64_t form) {
+  no_tangent(delta);
   return once({as_shape(gelu_backward_rows(flat(delta.detach(), "a cotangent"), values, codes, form), delta.sizes())},
               {delta.requires_grad()})[0];
 }
@@ -314,6 +323,9 @@ Tensor linear(const Tensor& x, const Tensor& weight, const optional<Tensor>& bia
     if (bias) b = bias->to(dtype);
     return at::linear(x.to(dtype), weight.to(dtype), b);
   }
+  no_tangent(x);
+  no_tangent(weight);
+  if (bias) no_tangent(*bias);
   if (values) return Linear::apply(x.to(dtype), weight, bias, *values, *codes);
   const Packed p = std::get<0>(pack_input(x, false));
   return Linear::apply(x.to(dtype), weight, bias, std::get<0>(p), std::get<1>(p));
@@ -351,6 +363,7 @@ struct Gelu : torch::autograd::Function<Gelu> {
 std::tuple<Tensor, optional<Packed>> gelu(const Tensor& x, int64_t form, bool pack_output, bool stats) {
   TORCH_CHECK_VALUE(x.dim() > 0, "an activation has at least one dimension");
   on_gpu(x);
+  no_tangent(x);
   if (at::GradMode::is_enabled() && x.requires_grad()) {
     const variable_list out = Gelu::apply(x, form, pack_output, stats);
     if (!pack_output) return {out[0], std::nullopt};

@@ -95,3 +95,27 @@ def test_operators_on_a_cotangent_with_a_gradient(dtype):
             got.float().sum().backward()
         with torch.no_grad():
             assert not call(delta.clone().requires_grad_(), packed).requires_grad
+
+
+# -------------------------------------------------- forward mode and tracing
+
+def test_tangents_are_refused():
+    """No operator carries a forward-mode tangent; none drops it."""
+    x, delta = activation(8, 64, torch.float32), cotangent(8, 64, torch.float32)
+    w = weight(16, 64)
+    packed = activations.pack(x)
+    calls = (activations.gelu, lambda t: activations.gelu(t, approximate="tanh", pack_output=True),
+             lambda t: activations.weight_gradient(t, packed), lambda t: activations.gelu_backward(t, packed),
+             lambda t: activations.linear(t, w), lambda t: activations.linear(x, w, t[0, :16]))
+    with torch.autograd.forward_ad.dual_level():
+        for leaf in (False, True):
+            dual = torch.autograd.forward_ad.make_dual(x.clone().requires_grad_(leaf), torch.ones_like(x))
+            for call in calls:
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(dual)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            activations.linear(x, torch.autograd.forward_ad.make_dual(w, torch.ones_like(w)))
+        # with a weight that takes no gradient, linear is torch's own layer
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        out = torch.autograd.forward_ad.unpack_dual(activations.linear(dual, w.detach()))
+        assert torch.equal(out.tangent, torch.nn.functional.linear(torch.ones_like(x), w.detach()))
