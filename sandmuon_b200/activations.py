@@ -18,7 +18,8 @@ package do so by themselves for every `PackedLinear` they select.
 
 `PackedLinear` is nn.Linear with a packed input.  Everything runs on CUDA
 (sm_100) tensors in float32, bfloat16 or float16; there is no CPU path.
-Forward-mode derivatives (torch.autograd.forward_ad) are refused.
+Forward-mode derivatives (torch.autograd.forward_ad) and tracing
+(torch.jit.trace, make_fx) are refused.
 """
 from __future__ import annotations
 

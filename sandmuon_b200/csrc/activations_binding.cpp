@@ -8,10 +8,12 @@
 // The library is opened by path (bind), so that another build of it can be
 // named at run time as for the ctypes binding.
 #include <ATen/autocast_mode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include "sandmuon_b200.h"
@@ -78,6 +80,15 @@ void on_gpu(const Tensor& t) {
 void no_tangent(const Tensor& t) {
   TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(),
                               "sandmuon_b200.activations has no forward-mode derivatives");
+}
+
+// A trace (torch.jit.trace, make_fx) records the torch operators that run: the
+// allocation of an output, and not the kernel that fills it.
+void no_trace() {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                  !(Modes::any_modes_set() && Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY)),
+              "functions of sandmuon_b200.activations cannot be traced");
 }
 
 std::string text(const Tensor& t) {
@@ -158,9 +169,13 @@ Packed pack_rows(const Tensor& x, bool stats) {
   return {values, codes, sums};
 }
 
-Packed pack(const Tensor& x, bool stats) { return pack_rows(flat(x.detach(), "an activation"), stats); }
+Packed pack(const Tensor& x, bool stats) {
+  no_trace();
+  return pack_rows(flat(x.detach(), "an activation"), stats);
+}
 
 Tensor unpack(const Tensor& values, const Tensor& codes, at::IntArrayRef shape, at::ScalarType dtype) {
+  no_trace();
   const int code = code_of(dtype, "the unpacked type");
   on_gpu(values);
   const c10::cuda::CUDAGuard guard(values.device());
@@ -190,6 +205,7 @@ Tensor weight_gradient_rows(const Tensor& delta, const Tensor& values, const Ten
 
 Tensor weight_gradient(const Tensor& delta, const Tensor& values, const Tensor& codes, int64_t d_in,
                        at::ScalarType dtype) {
+  no_trace();
   no_tangent(delta);
   return once({weight_gradient_rows(flat(delta.detach(), "a cotangent"), values, codes, d_in, dtype)},
               {delta.requires_grad()})[0];
@@ -248,6 +264,7 @@ Tensor gelu_backward_rows(const Tensor& delta, const Tensor& values, const Tenso
 Tensor as_shape(const Tensor& t, at::IntArrayRef shape) { return t.sizes() == shape ? t : t.view(shape); }
 
 Tensor gelu_backward(const Tensor& delta, const Tensor& values, const Tensor& codes, int64_t form) {
+  no_trace();
   no_tangent(delta);
   return once({as_shape(gelu_backward_rows(flat(delta.detach(), "a cotangent"), values, codes, form), delta.sizes())},
               {delta.requires_grad()})[0];
@@ -323,6 +340,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const optional<Tensor>& bia
     if (bias) b = bias->to(dtype);
     return at::linear(x.to(dtype), weight.to(dtype), b);
   }
+  no_trace();
   no_tangent(x);
   no_tangent(weight);
   if (bias) no_tangent(*bias);
@@ -363,6 +381,7 @@ struct Gelu : torch::autograd::Function<Gelu> {
 std::tuple<Tensor, optional<Packed>> gelu(const Tensor& x, int64_t form, bool pack_output, bool stats) {
   TORCH_CHECK_VALUE(x.dim() > 0, "an activation has at least one dimension");
   on_gpu(x);
+  no_trace();
   no_tangent(x);
   if (at::GradMode::is_enabled() && x.requires_grad()) {
     const variable_list out = Gelu::apply(x, form, pack_output, stats);

@@ -5,6 +5,7 @@ An operator that cannot give what is asked of it raises; it never returns a
 constant in its place."""
 import pytest
 import torch
+import torch.fx.experimental.proxy_tensor
 
 from sandmuon_b200 import activations
 from test_gpu_activations import DTYPES, activation, cotangent
@@ -119,3 +120,22 @@ def test_tangents_are_refused():
         dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
         out = torch.autograd.forward_ad.unpack_dual(activations.linear(dual, w.detach()))
         assert torch.equal(out.tangent, torch.nn.functional.linear(torch.ones_like(x), w.detach()))
+
+
+def test_tracing_is_refused():
+    """A trace would record the allocation of an output and not the kernel that
+    fills it."""
+    make_fx = torch.fx.experimental.proxy_tensor.make_fx
+    x, w = activation(8, 64, torch.float32), weight(16, 64)
+    packed = activations.pack(x)
+    calls = (activations.gelu, lambda t: activations.pack(t).values, lambda t: activations.pack_input(t).values,
+             lambda t: activations.unpack(packed) + t, lambda t: activations.weight_gradient(t, packed),
+             lambda t: activations.gelu_backward(t, packed), lambda t: activations.linear(t, w))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(call, x, check_trace=False)
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(lambda t: call(t))(x)
+    frozen = w.detach()
+    traced = torch.jit.trace(lambda t: activations.linear(t, frozen), x)  # torch's own layer
+    assert torch.equal(traced(2 * x), torch.nn.functional.linear(2 * x, frozen))
