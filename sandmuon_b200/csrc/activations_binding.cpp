@@ -230,13 +230,15 @@ struct GeluOut {
   optional<Tensor> in_values, in_codes, out_values, out_codes, sums;
 };
 
-GeluOut gelu_rows(const Tensor& x, int64_t form, bool keep_input, bool pack_output, bool stats) {
+// x: the rows of an activation of the given shape, which y takes.
+GeluOut gelu_rows(const Tensor& x, at::IntArrayRef shape, int64_t form, bool keep_input, bool pack_output,
+                  bool stats) {
   const int code = code_of(x.scalar_type(), "an activation");
   on_gpu(x);
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t rows = x.size(0), cols = x.size(1);
   GeluOut o;
-  o.y = at::empty({rows, cols}, x.options());
+  o.y = at::empty(shape, x.options());
   if (keep_input) o.in_values = new_values(x, rows, cols), o.in_codes = new_codes(x, rows, cols);
   if (pack_output) o.out_values = new_values(x, rows, cols), o.out_codes = new_codes(x, rows, cols);
   if (stats) o.sums = at::empty({2, cols}, x.options().dtype(at::kFloat));
@@ -282,7 +284,9 @@ struct Linear : torch::autograd::Function<Linear> {
     ctx->saved_data["x_grad"] = x.requires_grad();
     optional<Tensor> b;
     if (bias) b = bias->to(dtype);
-    return at::linear(x, cast, b);
+    // a view would not let in-place operations (an activation, a residual) at it
+    const Tensor y = at::linear(x, cast, b);
+    return y.is_view() ? at::_unsafe_view(y, y.sizes()) : y;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -351,10 +355,10 @@ Tensor linear(const Tensor& x, const Tensor& weight, const optional<Tensor>& bia
 
 struct Gelu : torch::autograd::Function<Gelu> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, int64_t form, bool pack_output, bool stats) {
-    GeluOut o = gelu_rows(flat(x, "an activation"), form, true, pack_output, stats);
+    GeluOut o = gelu_rows(flat(x, "an activation"), x.sizes(), form, true, pack_output, stats);
     ctx->save_for_backward({*o.in_values, *o.in_codes});
     ctx->saved_data["form"] = form;
-    variable_list out{as_shape(o.y, x.sizes())};
+    variable_list out{o.y};
     if (pack_output) {
       variable_list plain{*o.out_values, *o.out_codes};
       if (stats) plain.push_back(*o.sums);
@@ -388,10 +392,9 @@ std::tuple<Tensor, optional<Packed>> gelu(const Tensor& x, int64_t form, bool pa
     if (!pack_output) return {out[0], std::nullopt};
     return {out[0], Packed(out[1], out[2], stats ? optional<Tensor>(out[3]) : std::nullopt)};
   }
-  GeluOut o = gelu_rows(flat(x.detach(), "an activation"), form, false, pack_output, stats);
-  const Tensor y = as_shape(o.y, x.sizes());
-  if (!pack_output) return {y, std::nullopt};
-  return {y, Packed(*o.out_values, *o.out_codes, o.sums)};
+  GeluOut o = gelu_rows(flat(x.detach(), "an activation"), x.sizes(), form, false, pack_output, stats);
+  if (!pack_output) return {o.y, std::nullopt};
+  return {o.y, Packed(*o.out_values, *o.out_codes, o.sums)};
 }
 
 }  // namespace

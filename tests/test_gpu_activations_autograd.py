@@ -139,3 +139,48 @@ def test_tracing_is_refused():
     frozen = w.detach()
     traced = torch.jit.trace(lambda t: activations.linear(t, frozen), x)  # torch's own layer
     assert torch.equal(traced(2 * x), torch.nn.functional.linear(2 * x, frozen))
+
+
+# ------------------------------------------------------------ in-place changes
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(48,), (5, 48), (2, 5, 48), (2, 3, 5, 48), (0, 48)])
+def test_outputs_can_be_changed_in_place(shape, dtype):
+    """relu_, residual additions and scalings of an output, as after nn.Linear."""
+    base = torch.randn(*shape, generator=torch.Generator().manual_seed(3)).to(dtype).to(DEV)
+    w = weight(32, 48)
+    b = torch.zeros(32, device=DEV, requires_grad=True)
+    for bias in (None, b):
+        x = base.clone().requires_grad_()
+        want = torch.nn.functional.linear(x, w.to(dtype), None if bias is None else bias.to(dtype)).detach()
+        y = activations.linear(x, w, bias)
+        y += 1
+        y.relu_()
+        assert torch.equal(y, (want + 1).relu())
+        y.sum().backward()
+        kept = (want + 1 > 0).to(dtype)
+        assert torch.equal(x.grad, (kept.reshape(-1, 32) @ w.detach().to(dtype)).view(shape))
+        assert torch.equal(w.grad, activations.weight_gradient(kept, activations.pack(base)))
+        w.grad = None
+    for pack_output in (False, True):
+        x = base.clone().requires_grad_()
+        y = activations.gelu(x, pack_output=pack_output)
+        y = y[0] if pack_output else y
+        want = y.detach().clone()
+        y.mul_(2)
+        y += 1
+        assert torch.equal(y, want * 2 + 1)
+        y.sum().backward()
+        assert torch.equal(x.grad, activations.gelu_backward(torch.full_like(base, 2), activations.pack(base)))
+
+
+def test_inplace_modules_after_a_packed_layer():
+    layer = activations.PackedLinear(48, 32).to(DEV)
+    plain = torch.nn.Linear(48, 32).to(DEV)
+    plain.load_state_dict(layer.state_dict())
+    x = activation(10, 48, torch.float32).view(2, 5, 48)
+    outs = [torch.nn.Sequential(m, torch.nn.ReLU(inplace=True))(x) for m in (layer, plain)]
+    assert torch.equal(*outs)
+    outs[0].sum().backward()
+    outs[1].sum().backward()
+    assert torch.equal(layer.bias.grad, plain.bias.grad)
