@@ -277,6 +277,7 @@ struct Linear : torch::autograd::Function<Linear> {
                         const Tensor& values, const Tensor& codes) {
     const at::ScalarType dtype = x.scalar_type();
     const Tensor cast = weight.to(dtype);
+    ctx->set_materialize_grads(false);
     ctx->save_for_backward({cast, values, codes});
     ctx->saved_data["weight"] = static_cast<int64_t>(weight.scalar_type());
     ctx->saved_data["bias"] = static_cast<int64_t>(bias ? bias->scalar_type() : at::kFloat);
@@ -290,8 +291,9 @@ struct Linear : torch::autograd::Function<Linear> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const bool delta_grad = grads[0].requires_grad();
     variable_list out(5);
+    if (!grads[0].defined()) return out;
+    const bool delta_grad = grads[0].requires_grad();
     {
       const at::NoGradGuard no_grad;
       const variable_list saved = ctx->get_saved_variables();
@@ -356,6 +358,8 @@ Tensor linear(const Tensor& x, const Tensor& weight, const optional<Tensor>& bia
 struct Gelu : torch::autograd::Function<Gelu> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, int64_t form, bool pack_output, bool stats) {
     GeluOut o = gelu_rows(flat(x, "an activation"), x.sizes(), form, true, pack_output, stats);
+    // no zeros in place of the gradients that y's checkpoint and sums never have
+    ctx->set_materialize_grads(false);
     ctx->save_for_backward({*o.in_values, *o.in_codes});
     ctx->saved_data["form"] = form;
     variable_list out{o.y};
@@ -370,6 +374,7 @@ struct Gelu : torch::autograd::Function<Gelu> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(4);
+    if (!grads[0].defined()) return out;
     {
       const at::NoGradGuard no_grad;
       const variable_list saved = ctx->get_saved_variables();

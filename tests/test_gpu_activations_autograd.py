@@ -184,3 +184,45 @@ def test_inplace_modules_after_a_packed_layer():
     outs[0].sum().backward()
     outs[1].sum().backward()
     assert torch.equal(layer.bias.grad, plain.bias.grad)
+
+
+# --------------------------------------------------------------------- memory
+
+def test_backward_of_gelu_allocates_its_result_alone():
+    """No zero gradients for the output's checkpoint and sums, which take
+    none."""
+    x = activation(4096, 4096, torch.bfloat16).requires_grad_()
+    delta = cotangent(4096, 4096, torch.bfloat16)
+    for stats in (False, True):
+        y, packed = activations.gelu(x, pack_output=True, stats=stats)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        dx, = torch.autograd.grad(y, x, delta)
+        used = torch.cuda.max_memory_allocated() - before
+        # dx and allocation granularity; the checkpoint would add half of dx again
+        assert used <= dx.numel() * dx.element_size() + (1 << 20)
+        del y, packed, dx
+
+
+def test_a_gradient_that_nothing_gives():
+    """A cotangent that is left undefined behind an output stays so, as with
+    torch's own layers."""
+    class Nothing(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, y):
+            return y.clone()
+
+        @staticmethod
+        def backward(ctx, delta):
+            return None
+
+    w = weight(32, 48)
+    b = torch.zeros(32, device=DEV, requires_grad=True)
+    calls = (lambda x: activations.linear(x, w, b), activations.gelu,
+             lambda x: activations.gelu(x, pack_output=True, stats=True)[0])
+    for call in calls:
+        x = activation(10, 48, torch.float32).requires_grad_()
+        assert torch.autograd.grad(Nothing.apply(call(x)).sum(), x, allow_unused=True) == (None,)
+        Nothing.apply(call(x)).sum().backward()
+        assert w.grad is None and b.grad is None
