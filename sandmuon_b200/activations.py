@@ -117,7 +117,8 @@ def pack(x: torch.Tensor, *, stats: bool = False) -> PackedActivation:
 def pack_input(x: torch.Tensor, *, stats: bool = False) -> PackedActivation:
     """The checkpoint that linear layers reading x take under the current
     autocast state: of x as it comes, or of its float16 values where the layers
-    compute in float16 (their cotangents then need those)."""
+    compute in float16 (their cotangents then need those).  stats: the column
+    sums of x as it comes, as the optimizers' hooks of plain layers take them."""
     parts, half = _lib.binding().pack_input(x, stats)
     return PackedActivation._made(parts, x.shape, torch.float16 if half else x.dtype)
 

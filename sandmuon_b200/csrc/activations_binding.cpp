@@ -211,9 +211,11 @@ Tensor weight_gradient(const Tensor& delta, const Tensor& values, const Tensor& 
               {delta.requires_grad()})[0];
 }
 
-// delta.float().sum(0): the column sums of the statistics kernels.
-Tensor column_sums(const Tensor& rows) {
-  const int code = code_of(rows.scalar_type(), "a cotangent");
+// [2, columns]: column sums of the squares and of the values, by the statistics
+// kernels of the plain layers' hooks.
+Tensor column_statistics(const Tensor& rows, const char* what) {
+  const int code = rows.scalar_type() == at::kDouble ? SM_DTYPE_F64 : code_of(rows.scalar_type(), what);
+  on_gpu(rows);
   const c10::cuda::CUDAGuard guard(rows.device());
   const int64_t n = rows.size(1);
   Tensor both = at::zeros({2, n}, rows.options().dtype(at::kFloat));
@@ -222,8 +224,11 @@ Tensor column_sums(const Tensor& rows) {
   check(api.stats_accumulate(rows.data_ptr(), code, rows.size(0), n, rows.stride(0), rows.stride(1), sq, sq + n,
                              ws.ptr(), ws.n, stream_of(rows)),
         "sm_stats_accumulate");
-  return both.select(0, 1);
+  return both;
 }
+
+// delta.float().sum(0)
+Tensor column_sums(const Tensor& rows) { return column_statistics(rows, "a cotangent").select(0, 1); }
 
 struct GeluOut {
   Tensor y;
@@ -315,10 +320,14 @@ at::ScalarType compute_type(const Tensor& x) {
   return at::autocast::is_autocast_enabled(at::kCUDA) ? at::autocast::get_autocast_dtype(at::kCUDA) : x.scalar_type();
 }
 
-// and whether it is of float16 values
+// and whether it is of float16 values.  The sums are always those of x itself:
+// where it was rounded to float16 they take a read of their own.
 std::tuple<Packed, bool> pack_input(const Tensor& x, bool stats) {
   const bool half = compute_type(x) == at::kHalf;
-  return {pack(half ? x.detach().to(at::kHalf) : x, stats), half};
+  const bool rounded = half && x.scalar_type() != at::kHalf;
+  Packed p = pack(rounded ? x.detach().to(at::kHalf) : x, stats && !rounded);
+  if (stats && rounded) std::get<2>(p) = column_statistics(flat(x.detach(), "an activation"), "an activation");
+  return {p, half};
 }
 
 // packed_cols, packed_half: of the given checkpoint (values, codes), if any

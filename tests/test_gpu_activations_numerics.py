@@ -1,0 +1,64 @@
+"""Numerics of the 8-bit checkpoint operators beyond single calls: statistics
+under autocast.
+
+Tolerances, from the arithmetic: an FP32 chain of n additions of terms of one
+sign is off by at most n * 2^-24 relative; FP64 joins add one rounding to FP32."""
+import numpy as np
+import pytest
+import torch
+
+from sandmuon_b200 import DiagonalWeightedPE, RankOneAWeightedPE, activations
+from test_gpu_activations import check_sums, f64
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+
+
+# ------------------------------------------------------------------ statistics
+
+def between_halves(rows, cols):
+    """FP32 values that FP16 rounds all the same way (by 2^-12 relative), and
+    some that it cannot hold."""
+    x = torch.full((rows, cols), 1 + 2.0 ** -12, device=DEV)
+    x[:, ::3] *= -1
+    return x
+
+
+@pytest.mark.parametrize("cols", [40, 128])
+def test_statistics_under_autocast_are_of_the_input_itself(cols):
+    """FP16 layers keep a checkpoint of the FP16 values; the column sums are
+    those of the FP32 input, as a plain layer's hook takes them."""
+    x = between_halves(64, cols)
+    x[3, 1], x[5, 2] = 7e4, -3e5  # past FP16's range
+    for dtype in (torch.float16, torch.bfloat16):
+        with torch.autocast("cuda", dtype=dtype):
+            packed = activations.pack_input(x, stats=True)
+            assert activations.pack_input(x).sums is None
+        source = x.half() if dtype == torch.float16 else x
+        assert packed.dtype == source.dtype
+        plain = activations.pack(source)
+        assert torch.equal(packed.values, plain.values) and torch.equal(packed.exponents, plain.exponents)
+        check_sums(packed.sums, x)
+    for shape in ((0, cols), (2, 0, cols), (cols,)):
+        with torch.autocast("cuda", dtype=torch.float16):
+            packed = activations.pack_input(torch.ones(shape, device=DEV), stats=True)
+        assert packed.shape == shape and packed.sums.shape == (2, cols)
+        assert torch.equal(packed.sums, torch.full((2, cols), float(shape == (cols,)), device=DEV))
+
+
+@pytest.mark.parametrize("rank_one", [True, False])
+def test_hook_statistics_of_packed_and_plain_layers_agree_under_autocast(rank_one):
+    """150 terms of one sign: both sums are within 158 * 2^-24 of the exact one."""
+    x = between_halves(150, 64)
+    make = RankOneAWeightedPE if rank_one else DiagonalWeightedPE
+    keys = ("a_sum", "a_first_sum") if rank_one else ("a_sum",)
+    seen = []
+    for layer in (torch.nn.Linear(64, 48), activations.PackedLinear(64, 48)):
+        model = torch.nn.Sequential(layer).to(DEV)
+        opt = make(model, lr=1e-2)
+        with torch.autocast("cuda", dtype=torch.float16):
+            model(x).float().sum().backward()
+        seen.append([f64(opt.state[layer.weight][k]) for k in keys])
+        opt.close()
+    for a, b in zip(*seen):
+        assert (np.abs(a - b) <= 2 * 158 * 2.0 ** -24 * np.abs(a)).all()
