@@ -25,10 +25,15 @@ struct ActLaunch {
   int splits;
 };
 
+// Rows that a lane adds to its column sums in FP32 before the FP64 join: about the
+// length of the chains of the statistics kernels, whose place these sums take.
+constexpr int kSumChain = 128;
+
 // CTAs of 256 threads: strips of up to 256 columns times enough row ranges for
 // one wave of `ctas` CTAs per SM, each range of whole passes.  Up to four
 // passes stay in one range: a second launch to join column sums costs more.
-static ActLaunch act_launch(int64_t rows, int64_t cols, bool vec, int sms, int ctas) {
+// `sums`: the launch takes column sums; tall inputs then get more ranges.
+static ActLaunch act_launch(int64_t rows, int64_t cols, bool vec, int sms, int ctas, bool sums) {
   ActLaunch l;
   const int64_t padded = act_lde(cols) * kGroup;
   int log_lanes = 2;
@@ -39,7 +44,10 @@ static ActLaunch act_launch(int64_t rows, int64_t cols, bool vec, int sms, int c
   const int64_t want = std::max<int64_t>(1, static_cast<int64_t>(ctas) * sms / strips);
   const int64_t most = rows <= 4 * per_pass ? 1 : cdiv(rows, per_pass);
   int64_t splits = std::min<int64_t>(std::min(want, most), 65535);
-  const int64_t rows_per_cta = round_up(cdiv(rows, splits), per_pass);
+  int64_t rows_per_cta = round_up(cdiv(rows, splits), per_pass);
+  if (sums)
+    rows_per_cta = std::min(rows_per_cta, std::max<int64_t>(kSumChain * (kActThreads >> log_lanes),
+                                                            round_up(cdiv(rows, 65535), per_pass)));
   splits = std::max<int64_t>(1, cdiv(rows, rows_per_cta));
   l.g.rows = rows;
   l.g.cols = cols;
@@ -263,8 +271,8 @@ size_t sm_activation_sums_workspace_bytes(int64_t n_rows, int64_t n_cols) {
   DeviceInfo* di;
   if (current_device_info(&di) == SM_OK) sms = di->sms;
   constexpr int kCtas = std::max(kPackCtas, kGeluForwardCtas);
-  const int splits = std::max(act_launch(n_rows, n_cols, true, sms, kCtas).splits,
-                              act_launch(n_rows, n_cols, false, sms, kCtas).splits);
+  const int splits = std::max(act_launch(n_rows, n_cols, true, sms, kCtas, true).splits,
+                              act_launch(n_rows, n_cols, false, sms, kCtas, true).splits);
   return splits == 1 ? 0 : static_cast<size_t>(splits) * 2 * static_cast<size_t>(n_cols) * sizeof(float);
 }
 
@@ -283,7 +291,7 @@ int sm_activation_pack(const void* x, int dtype, int64_t n_rows, int64_t n_cols,
   DeviceInfo* di;
   SM_TRY(current_device_info(&di));
   const bool vec = vec8_rows(x, dtype, n_rows, n_cols, row_stride, col_stride);
-  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms, kPackCtas);
+  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms, kPackCtas, sums != nullptr);
   const Checkpoint c = act_checkpoint(values, exponents, n_cols);
   float* target = nullptr;
   SM_TRY(act_sums_target(l, sums, workspace, workspace_bytes, &target));
@@ -305,7 +313,7 @@ int sm_activation_unpack(const int8_t* values, const uint8_t* exponents, int64_t
   SM_TRY(current_device_info(&di));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool vec = vec8_rows(out, dtype, n_rows, n_cols, n_cols, 1);
-  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms, kUnpackCtas);
+  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms, kUnpackCtas, false);
   const Checkpoint c = act_checkpoint(values, exponents, n_cols);
   if (dtype == SM_DTYPE_F32) return unpack_run(l, c, static_cast<float*>(out), vec, st);
   if (dtype == SM_DTYPE_BF16) return unpack_run(l, c, static_cast<__nv_bfloat16*>(out), vec, st);
@@ -331,7 +339,7 @@ int sm_gelu_forward(const void* x, int dtype, int64_t n_rows, int64_t n_cols, in
   SM_TRY(current_device_info(&di));
   const bool vec = vec8_rows(x, dtype, n_rows, n_cols, row_stride, col_stride) &&
                    vec8_rows(y, dtype, n_rows, n_cols, n_cols, 1);
-  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms, kGeluForwardCtas);
+  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms, kGeluForwardCtas, sums != nullptr);
   const Checkpoint in = act_checkpoint(in_values, in_exponents, n_cols);
   const Checkpoint out = act_checkpoint(out_values, out_exponents, n_cols);
   float* target = nullptr;
@@ -361,7 +369,7 @@ int sm_gelu_backward(const void* delta, int dtype, int64_t n_rows, int64_t n_col
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool vec = vec8_rows(delta, dtype, n_rows, n_cols, row_stride, col_stride) &&
                    vec8_rows(dx, dtype, n_rows, n_cols, n_cols, 1);
-  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms, kGeluBackwardCtas);
+  const ActLaunch l = act_launch(n_rows, n_cols, vec, di->sms, kGeluBackwardCtas, false);
   const Checkpoint c = act_checkpoint(values, exponents, n_cols);
   const bool th = form == SM_GELU_TANH;
   if (dtype == SM_DTYPE_F32)

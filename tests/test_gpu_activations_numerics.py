@@ -1,5 +1,5 @@
 """Numerics of the 8-bit checkpoint operators beyond single calls: statistics
-under autocast.
+under autocast, long column sums.
 
 Tolerances, from the arithmetic: an FP32 chain of n additions of terms of one
 sign is off by at most n * 2^-24 relative; FP64 joins add one rounding to FP32."""
@@ -62,3 +62,21 @@ def test_hook_statistics_of_packed_and_plain_layers_agree_under_autocast(rank_on
         opt.close()
     for a, b in zip(*seen):
         assert (np.abs(a - b) <= 2 * 158 * 2.0 ** -24 * np.abs(a)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_column_sums_of_a_tall_and_wide_input(dtype):
+    """A lane adds at most 128 rows in FP32 before the FP64 join, whatever the
+    shape: equal terms, whose rounding errors add up, stay within 132 * 2^-24.
+    (One broadcast row: the input itself takes no memory.)"""
+    rows, cols = 16384, 131072
+    row = (torch.arange(cols, device=DEV) % 977 + 300).float().mul_(0.001).to(dtype)
+    x = row.expand(rows, cols)
+    packed = activations.pack(x, stats=True)
+    v = row.double()
+    want = torch.stack((v * v, v)) * rows
+    assert float(((packed.sums.double() - want).abs() / want).max()) <= 132 * 2.0 ** -24
+    del packed
+    odd = row[1:].expand(rows, cols - 1)  # the element mapping
+    sums = activations.pack(odd, stats=True).sums
+    assert float(((sums.double() - want[:, 1:]).abs() / want[:, 1:]).max()) <= 132 * 2.0 ** -24
