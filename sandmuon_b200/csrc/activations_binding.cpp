@@ -413,15 +413,22 @@ std::tuple<Tensor, optional<Packed>> gelu(const Tensor& x, int64_t form, bool pa
 
 }  // namespace
 
+// Without Python's lock: an allocation or a launch may wait for the GPU, and
+// other threads (the one that a collective waits for among them) run meanwhile.
+using Unlocked = pybind11::call_guard<pybind11::gil_scoped_release>;
+
 PYBIND11_MODULE(_activations, m) {
   m.def("bind", &bind);
-  m.def("pack", &pack);
-  m.def("pack_input", &pack_input);
-  m.def("unpack", [](const Tensor& values, const Tensor& codes, const std::vector<int64_t>& shape, at::ScalarType dtype) {
-    return unpack(values, codes, shape, dtype);
-  });
-  m.def("weight_gradient", &weight_gradient);
-  m.def("linear", &linear);
-  m.def("gelu", &gelu);
-  m.def("gelu_backward", &gelu_backward);
+  m.def("pack", &pack, Unlocked());
+  m.def("pack_input", &pack_input, Unlocked());
+  m.def(
+      "unpack",
+      [](const Tensor& values, const Tensor& codes, const std::vector<int64_t>& shape, at::ScalarType dtype) {
+        return unpack(values, codes, shape, dtype);
+      },
+      Unlocked());
+  m.def("weight_gradient", &weight_gradient, Unlocked());
+  m.def("linear", &linear, Unlocked());
+  m.def("gelu", &gelu, Unlocked());
+  m.def("gelu_backward", &gelu_backward, Unlocked());
 }
