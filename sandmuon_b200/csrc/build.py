@@ -74,21 +74,29 @@ def binding_command(out: Path) -> list[str]:
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compiles the library and the extension, each unless it is newer than
     every file it is made from; returns the library's path."""
+    # every command is there before the first compiler starts
     jobs = []
     for target, depends, command in (
             (LIB_PATH, DEPENDS,
              lambda out: [nvcc_path(), *NVCC_FLAGS, "-I", str(ROOT / "include"), "-o", str(out), *map(str, SOURCES)]),
             (BINDING_PATH, BINDING_DEPENDS, binding_command)):
-        if not force and up_to_date(target, depends):
-            continue
-        tmp = target.with_suffix(".so.tmp")
-        cmd = command(tmp)
-        if verbose:
-            print(" ".join(cmd), file=sys.stderr)
-        jobs.append((target, tmp, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+        if force or not up_to_date(target, depends):
+            tmp = target.with_suffix(".so.tmp")
+            jobs.append((target, tmp, command(tmp)))
+    processes = []
+    try:
+        for _, _, cmd in jobs:
+            if verbose:
+                print(" ".join(cmd), file=sys.stderr)
+            processes.append(subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))
+        outputs = [process.communicate()[0] for process in processes]
+    finally:
+        for process in processes:
+            if process.poll() is None:
+                process.kill()
+                process.wait()
     failed = []
-    for target, tmp, process in jobs:
-        output = process.communicate()[0]
+    for (target, tmp, _), process, output in zip(jobs, processes, outputs):
         if process.returncode != 0:
             failed.append(f"building {target.name} failed ({process.returncode}):\n{output}")
             continue
