@@ -9,6 +9,7 @@ import ctypes
 import importlib.machinery
 import importlib.util
 import os
+import sys
 import threading
 from pathlib import Path
 
@@ -160,8 +161,15 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
-BINDING_PATH = Path(__file__).resolve().parent / "_activations.so"
 _binding = None
+
+
+def binding_path() -> Path:
+    """Where the torch extension of this Python and torch lies.  Its name says
+    what it was built for: it uses torch's C++ interface, which differs between
+    versions, and travels with the tree."""
+    tag = f"{sys.implementation.cache_tag}-torch-{torch.__version__}-abi{int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+    return Path(__file__).resolve().parent / f"_activations.{tag}.so"
 
 
 def binding():
@@ -173,11 +181,12 @@ def binding():
     load()
     with _lib_lock:
         if _binding is None:
-            if not BINDING_PATH.exists():
+            path = binding_path()
+            if not path.exists():
                 raise RuntimeError(
-                    f"sandmuon_b200: {BINDING_PATH.name} is not built; run `python -m sandmuon_b200.csrc.build` "
+                    f"sandmuon_b200: {path.name} is not built; run `python -m sandmuon_b200.csrc.build` "
                     "(there is no CPU fallback)")
-            loader = importlib.machinery.ExtensionFileLoader("_activations", str(BINDING_PATH))
+            loader = importlib.machinery.ExtensionFileLoader("_activations", str(path))
             module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_activations", loader))
             loader.exec_module(module)
             module.bind(str(LIB_PATH))

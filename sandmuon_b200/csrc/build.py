@@ -3,9 +3,9 @@ the activation operators with g++, in-tree.
 
 Usage:  python -m sandmuon_b200.csrc.build   (or sandmuon_b200.csrc.build.build())
 
-The shared objects land in the package (sandmuon_b200/libsandmuon_b200.so,
-sandmuon_b200/_activations.so) so they travel with the source tree; nothing is
-installed into site-packages.
+The shared objects land in the package (libsandmuon_b200.so, and
+_activations.<python>-torch-<version>-abi<n>.so) so they travel with the source
+tree; nothing is installed into site-packages.
 """
 from __future__ import annotations
 
@@ -15,6 +15,8 @@ import subprocess
 import sys
 import sysconfig
 from pathlib import Path
+
+from .._lib import binding_path
 
 CSRC = Path(__file__).resolve().parent
 PACKAGE = CSRC.parent
@@ -26,7 +28,6 @@ DEPENDS = SOURCES + [CSRC / "sm_common.cuh", CSRC / "sm_gemm.cuh", CSRC / "sm_ke
                      CSRC / "sm_activation.cuh", CSRC / "sm_wgrad.cuh", CSRC / "sm_activation_host.cuh",
                      ROOT / "include" / "sandmuon_b200.h"]
 
-BINDING_PATH = PACKAGE / "_activations.so"
 BINDING_SOURCE = CSRC / "activations_binding.cpp"
 BINDING_DEPENDS = [BINDING_SOURCE, ROOT / "include" / "sandmuon_b200.h"]
 
@@ -79,7 +80,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     for target, depends, command in (
             (LIB_PATH, DEPENDS,
              lambda out: [nvcc_path(), *NVCC_FLAGS, "-I", str(ROOT / "include"), "-o", str(out), *map(str, SOURCES)]),
-            (BINDING_PATH, BINDING_DEPENDS, binding_command)):
+            (binding_path(), BINDING_DEPENDS, binding_command)):
         if force or not up_to_date(target, depends):
             tmp = target.with_suffix(".so.tmp")
             jobs.append((target, tmp, command(tmp)))

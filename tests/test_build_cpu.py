@@ -40,3 +40,19 @@ def test_no_compiler_is_left_behind_when_another_does_not_start(compilers, tmp_p
         build.build(force=True)
     time.sleep(0.5)
     assert not alive(compilers)
+
+
+def test_the_extension_of_another_torch_is_not_taken(built_library, monkeypatch):
+    """The extension is kept and loaded for the torch it was built with alone."""
+    from sandmuon_b200 import _lib
+    asked = []
+    monkeypatch.setattr(build, "binding_command", lambda out: asked.append(out) or ["true"])
+    build.build()
+    assert not asked and _lib.binding() is not None
+    monkeypatch.setattr(build.os, "replace", lambda *_: None)
+    monkeypatch.setattr("torch.__version__", "0.0.0+other")
+    build.build()
+    assert len(asked) == 1 and "0.0.0+other" in asked[0].name
+    monkeypatch.setattr(_lib, "_binding", None)
+    with pytest.raises(RuntimeError, match="not built"):
+        _lib.binding()
