@@ -177,10 +177,17 @@ size_t sm_weight_gradient_workspace_bytes(const void* delta, int dtype, int64_t 
  * delta [n_rows, d_out] F32 / BF16 / F16 of any strides; the checkpoint is of
  * an [n_rows, d_in] input, packed from F16 if delta is F16.  Products are
  * exact and summed in FP32 on the tensor cores in an order that depends on the
- * sizes alone; out (F32 / BF16 / F16) is rounded once. */
+ * sizes alone; out (F32 / BF16 / F16) is rounded once.
+ * Should one of the kernel's bounded waits run out, the output tiles that it
+ * kept from their results are NaN and sm_device_status says so. */
 int sm_weight_gradient(const void* delta, int dtype, int64_t n_rows, int64_t d_out, int64_t row_stride,
                        int64_t col_stride, const int8_t* values, const uint8_t* exponents, int64_t d_in, void* out,
                        int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Fault injection for tests, on the host: in the weight gradients launched from
+ * now on, CTA pair `worker` does no work, as if its first wait had run out
+ * (negative: none, the default). */
+int sm_inject_expired_wait(int worker);
 
 /* ------------------------------------------------------ optimizer plan */
 

@@ -111,6 +111,7 @@ SIGNATURES = {
     "sm_weight_gradient_workspace_bytes": (_c_size, [_c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64]),
     "sm_weight_gradient": (_c_int, [_c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_void_p, _c_void_p, _c_i64,
                                     _c_void_p, _c_int, _c_void_p, _c_size, _c_void_p]),
+    "sm_inject_expired_wait": (_c_int, [_c_int]),
     "sm_plan_workspace_bytes": (_c_int, [ctypes.POINTER(SmPlanSpec), ctypes.POINTER(_c_size)]),
     "sm_plan_create": (_c_int, [ctypes.POINTER(SmPlanSpec), _c_void_p, _c_size, _c_void_p, ctypes.POINTER(_c_void_p)]),
     "sm_plan_step": (_c_int, [_c_void_p, ctypes.POINTER(SmStepArgs), _c_void_p]),

@@ -3,6 +3,8 @@
 // translation unit libsandmuon_b200.cu, which includes it last.
 #pragma once
 
+#include <atomic>
+
 namespace smb {
 
 static int64_t act_ld(int64_t cols) { return SM_ACTIVATION_LD(cols); }
@@ -146,6 +148,9 @@ static int gelu_backward_run(const T* d, int64_t rs, int64_t cs, bool vec, bool 
 }
 
 // ---------------------------------------------------------- weight gradient
+
+// WgradArgs::expired of the launches to come (sm_inject_expired_wait).
+static std::atomic<int> g_expired_worker{-1};
 
 // 2-D tensor map over rows of `stride` bytes.
 static int make_map_rows(CUtensorMap* m, CUtensorMapDataType type, const void* base, int64_t inner, int64_t outer,
@@ -449,10 +454,16 @@ int sm_weight_gradient(const void* delta, int dtype, int64_t n_rows, int64_t d_o
   wgrad_shares(g, &p);
   p.out = out;
   p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + g.plane_bytes);
+  p.expired = g_expired_worker.load();
   p.vec_out = aligned(out, 16) && (d_in * elem_size(out_dtype)) % 16 == 0;
   if (dtype == SM_DTYPE_F32) return wgrad_dispatch<3, false, 32>(out_dtype, p, !g.direct, g.partial, st);
   if (dtype == SM_DTYPE_BF16) return wgrad_dispatch<1, false, 64>(out_dtype, p, !g.direct, g.partial, st);
   return wgrad_dispatch<1, true, 64>(out_dtype, p, !g.direct, g.partial, st);
+}
+
+int sm_inject_expired_wait(int worker) {
+  g_expired_worker.store(worker < 0 ? -1 : worker);
+  return SM_OK;
 }
 
 }  // extern "C"

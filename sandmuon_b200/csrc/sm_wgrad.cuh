@@ -36,6 +36,10 @@
 // shared out by k-blocks (WgradArgs::parts).  A worker that holds only a part
 // of a tile leaves an FP32 partial tile, and k_wgrad_join adds those in worker
 // order (no atomics: results do not depend on timing).
+//
+// Every wait is bounded (kWaitTimeoutNs).  One that runs out sets the status
+// word, and whatever it kept from its result becomes NaN: `out` never shows
+// memory that was not written.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -89,6 +93,7 @@ struct WgradArgs {
   void* out;                // [d_out, d_in]
   float* partials;          // [2 * workers, kWgPartialFloats]
   int vec_out;              // rows of `out` take 16-byte stores
+  int expired;              // a worker whose first wait counts as run out, for tests; -1: none
 };
 
 // First k-block (counting through the shared tiles, end to end) of worker w,
@@ -422,6 +427,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int worker = static_cast<int>(blockIdx.x) / 2;
+  const bool live = worker != p.expired;
   const uint32_t smem_base = smem_u32(smem);
   const uint32_t bar_base = smem_u32(bars);
   // full (the leader's): delta bytes and converters of both CTAs.  done: the
@@ -451,7 +457,8 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
       mbar_init(bar_tfull(i), 1);
       mbar_init(bar_tempty(i), 2 * kWgEpiWarps);
     }
-    *abort_flag = 0;
+    *abort_flag = live ? 0 : kStatusTimeoutWgradProducer;
+    if (!live) atomicExch(&g_status, kStatusTimeoutWgradProducer);
     fence_barrier_init();
     fence_proxy_async_smem();
   }
@@ -480,7 +487,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
       WgRing<S::kAStages> ra;
       WgRing<S::kRing> rf, rd;  // this k-block, and the one kAStages back
       int64_t i = 0;
-      bool ok = true;
+      bool ok = live;
       for (WgIter it(p, worker); it.valid() && ok;) {
         const WgSegment s = it.get();
         const int mc = s.mi * kWgTileM + static_cast<int>(rank) * 128;
@@ -512,7 +519,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
     // (apart from delta's, whose waits for the MMAs would hold it back)
     if (lane == 0) {
       WgRing<S::kRawStages> rr;
-      bool ok = true;
+      bool ok = live;
       for (WgIter it(p, worker); it.valid() && ok;) {
         const WgSegment s = it.get();
         const int nc = s.ni * kWgTileN + static_cast<int>(rank) * 128;
@@ -535,7 +542,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
     // A lane copies the 4 codes of a token's 128 columns.  Codes outside the
     // checkpoint become 0: their values are 0 as well.
     WgRing<S::kRawStages> rr;
-    bool ok = true;
+    bool ok = live;
     for (WgIter it(p, worker); it.valid() && ok;) {
       const WgSegment s = it.get();
       const int g = (s.ni * kWgTileN + static_cast<int>(rank) * 128) / kGroup;
@@ -569,7 +576,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
       WgRing<S::kRing> rf;
       int home = 0;
       uint32_t uses0 = 0, uses1 = 0;  // chains that ran in each accumulator
-      bool ok = true, ready = false;
+      bool ok = live, ready = false;
       const uint64_t a_desc = umma_desc(slot_a(0), kChunkBytes, Swz::kSbo, Swz::kLayout);
       const uint64_t b_desc = umma_desc(slot_b(0), kChunkBytes, Swz::kSbo, Swz::kLayout);
       for (WgIter it(p, worker); it.valid() && ok; home ^= 1) {
@@ -642,8 +649,8 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
     };
     int home = 0;
     uint32_t uses0 = 0, uses1 = 0;
-    bool ok = true;
-    for (WgIter it(p, worker); it.valid() && ok; home ^= 1) {
+    bool ok = live;
+    for (WgIter it(p, worker); it.valid(); home ^= 1) {
       const WgSegment s = it.get();
       const bool whole = s.kb0 == 0 && s.kb1 == p.kblocks;
       const int row0 = s.mi * kWgTileM + static_cast<int>(rank) * 128 + quarter * 32;
@@ -652,7 +659,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
       const uint32_t t_home = t_row + static_cast<uint32_t>(home * kWgTileN);
       const uint32_t t_other = t_row + static_cast<uint32_t>((home ^ 1) * kWgTileN);
-      for (int begin = s.kb0; begin < s.kb1; begin += S::kChainBlocks) {
+      for (int begin = s.kb0; begin < s.kb1 && ok; begin += S::kChainBlocks) {
         const bool first = begin == s.kb0, last = begin + S::kChainBlocks >= s.kb1;
         const int acc = first ? home : home ^ 1;
         const uint32_t uses = acc ? uses1++ : uses0++;
@@ -721,6 +728,26 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
           }
         }
       }
+      if (!ok) {
+        // A wait ran out, here or (then this warp's own does too) before an MMA
+        // of the segment: its part of the result or partial tile becomes NaN,
+        // as do those of the segments that follow.
+        const float nan = __uint_as_float(0x7fffffffu);
+        if (!whole) {
+#pragma unroll 1
+          for (int col = kWgTileN / 2 * half; col < kWgTileN / 2 * (half + 1); col += 4)
+            *reinterpret_cast<float4*>(part + partial_offset(rank, quarter, col / 32, col / 4 % 8, lane)) =
+                make_float4(nan, nan, nan, nan);
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < 32 * (kWgTileN / 2 / 32); ++i) {
+            const int row = row0 + i / (kWgTileN / 2 / 32);
+            const int col = colt + kWgTileN / 2 * half + 32 * (i % (kWgTileN / 2 / 32)) + lane;
+            if (row < p.d_out && col < p.d_in)
+              static_cast<OUT*>(p.out)[static_cast<int64_t>(row) * p.d_in + col] = from_f32<OUT>(nan);
+          }
+        }
+      }
       it.next(s);
     }
   } else if (warp >= kWgConvWarp0) {
@@ -748,7 +775,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) k_wgrad(const __grid_constant__
     WgRing<S::kRing> rf, rd;  // this k-block, and the one kBStages back (from there on)
     // k-blocks of this worker: its share and its whole tiles
     const int64_t whole = p.shared + worker < p.tiles ? (p.tiles - 1 - p.shared - worker) / p.workers + 1 : 0;
-    const int64_t blocks = wgrad_begin(p, worker + 1) - wgrad_begin(p, worker) + whole * p.kblocks;
+    const int64_t blocks = live ? wgrad_begin(p, worker + 1) - wgrad_begin(p, worker) + whole * p.kblocks : 0;
     rr.slot = rb.slot = rf.slot = rd.slot = group;
     constexpr int kSkip = kWgConvGroups;
     static_assert(kSkip <= S::kBStages, "a group's first k-block finds its slot empty");

@@ -1,5 +1,6 @@
 """Numerics of the 8-bit checkpoint operators beyond single calls: statistics
-under autocast, long column sums.
+under autocast, long column sums, and what is left when a wait of the weight
+gradient runs out.
 
 Tolerances, from the arithmetic: an FP32 chain of n additions of terms of one
 sign is off by at most n * 2^-24 relative; FP64 joins add one rounding to FP32."""
@@ -7,8 +8,8 @@ import numpy as np
 import pytest
 import torch
 
-from sandmuon_b200 import DiagonalWeightedPE, RankOneAWeightedPE, activations
-from test_gpu_activations import check_sums, f64
+from sandmuon_b200 import DiagonalWeightedPE, RankOneAWeightedPE, _lib, activations
+from test_gpu_activations import DTYPES, activation, check_sums, cotangent, f64
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda:0")
@@ -80,3 +81,48 @@ def test_column_sums_of_a_tall_and_wide_input(dtype):
     odd = row[1:].expand(rows, cols - 1)  # the element mapping
     sums = activations.pack(odd, stats=True).sums
     assert float(((sums.double() - want[:, 1:]).abs() / want[:, 1:]).max()) <= 132 * 2.0 ** -24
+
+
+# ------------------------------------------------------ waits that run out
+
+@pytest.fixture
+def expired():
+    """Lets a worker (a CTA pair) of the following weight gradients take its
+    first wait as run out; the library does no work and waits for nothing
+    there, so nothing hangs."""
+    yield _lib.load().sm_inject_expired_wait
+    _lib.load().sm_inject_expired_wait(-1)
+    _lib.device_status(DEV)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,d_in,d_out", [
+    (300, 40, 24),         # one worker, one tile
+    (20000, 64, 300),      # two tiles in equal parts
+    (1100, 2048, 1280),    # stretches across tile borders
+    (2000, 2304, 2304),    # whole tiles and shared ones
+])
+def test_a_wait_that_ran_out_leaves_nan(rows, d_in, d_out, dtype, expired):
+    """Every element is the right one or NaN: no memory that was never written
+    is returned as a gradient, and the status word says what happened."""
+    x, delta = activation(rows, d_in, dtype), cotangent(rows, d_out, dtype)
+    packed = activations.pack(x)
+    for out_dtype in (torch.float32, torch.bfloat16):
+        want = activations.weight_gradient(delta, packed, dtype=out_dtype)
+        assert _lib.device_status(DEV) == 0
+        for worker in (0, 1, 5, 71):
+            assert expired(worker) == 0
+            # memory of the result: full of a value that is not the gradient's
+            torch.full((d_out, d_in), 7.0, dtype=out_dtype, device=DEV)
+            got = activations.weight_gradient(delta, packed, dtype=out_dtype)
+            assert expired(-1) == 0
+            bad = torch.isnan(got)
+            assert torch.equal(got[~bad], want[~bad])
+            assert (_lib.device_status(DEV) != 0) == bool(bad.any())
+            if worker == 0:
+                assert bad.any()
+            # whole 256 x 256 tiles
+            tiles = torch.nn.functional.max_pool2d(bad[None].float(), 256, ceil_mode=True)[0]
+            full = tiles.repeat_interleave(256, 0).repeat_interleave(256, 1)[:d_out, :d_in]
+            assert torch.equal(full > 0, bad)
+        assert torch.equal(activations.weight_gradient(delta, packed, dtype=out_dtype), want)
