@@ -97,9 +97,11 @@ std::string text(const Tensor& t) {
   return s + "]";
 }
 
-// [..., columns] as [rows, columns]
-Tensor flat(const Tensor& t, const char* what) {
-  TORCH_CHECK_VALUE(t.dim() > 0, what, " has at least one dimension");
+// [..., columns] as [rows, columns] whose memory holds the values (that of a
+// negative view, such as the imaginary part of a conjugate, does not).
+Tensor flat(const Tensor& given, const char* what) {
+  TORCH_CHECK_VALUE(given.dim() > 0, what, " has at least one dimension");
+  const Tensor t = given.is_neg() ? given.resolve_neg() : given;
   if (t.dim() == 2) return t;
   int64_t rows = 1;
   for (int64_t d = 0; d + 1 < t.dim(); ++d) rows *= t.size(d);

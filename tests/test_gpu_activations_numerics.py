@@ -1,6 +1,6 @@
 """Numerics of the 8-bit checkpoint operators beyond single calls: statistics
-under autocast, long column sums, and what is left when a wait of the weight
-gradient runs out.
+under autocast, long column sums, negative views, and what is left when a wait
+of the weight gradient runs out.
 
 Tolerances, from the arithmetic: an FP32 chain of n additions of terms of one
 sign is off by at most n * 2^-24 relative; FP64 joins add one rounding to FP32."""
@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from sandmuon_b200 import DiagonalWeightedPE, RankOneAWeightedPE, _lib, activations
-from test_gpu_activations import DTYPES, activation, check_sums, cotangent, f64
+from test_gpu_activations import DTYPES, activation, check_packed, check_sums, check_weight_gradient, cotangent, f64
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda:0")
@@ -126,3 +126,22 @@ def test_a_wait_that_ran_out_leaves_nan(rows, d_in, d_out, dtype, expired):
             full = tiles.repeat_interleave(256, 0).repeat_interleave(256, 1)[:d_out, :d_in]
             assert torch.equal(full > 0, bad)
         assert torch.equal(activations.weight_gradient(delta, packed, dtype=out_dtype), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_views_that_stand_for_their_negative(dtype):
+    """The imaginary part of a conjugate is a real tensor whose memory holds
+    the opposite sign."""
+    kind = torch.complex64 if dtype == torch.float32 else torch.complex32
+    base = activation(40, 64, dtype)
+    z = torch.zeros(40, 64, dtype=kind, device=DEV)
+    torch.view_as_real(z)[..., 1] = base
+    x = z.conj().imag
+    assert x.is_neg() and x.dtype == dtype
+    want = -base
+    packed = activations.pack(x, stats=True)
+    check_packed(packed, want)
+    check_sums(packed.sums, want)
+    check_weight_gradient(activations.weight_gradient(x, packed), want, packed)
+    assert torch.equal(activations.gelu(x), activations.gelu(want))
+    assert torch.equal(activations.gelu_backward(x, packed), activations.gelu_backward(want, packed))
