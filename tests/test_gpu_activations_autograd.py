@@ -226,3 +226,22 @@ def test_a_gradient_that_nothing_gives():
         assert torch.autograd.grad(Nothing.apply(call(x)).sum(), x, allow_unused=True) == (None,)
         Nothing.apply(call(x)).sum().backward()
         assert w.grad is None and b.grad is None
+
+
+# ------------------------------------------------- layers that share an input
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layers_that_share_an_input_give_the_input_gradient_of_plain_layers(dtype):
+    """Each layer's input gradient is rounded to the input's type and autograd
+    adds them there: bit for bit what as many plain layers give.  Repeated
+    passes give the same bits."""
+    ws = [weight(96, 80, seed) for seed in range(3)]
+    base = activation(500, 80, dtype)
+    deltas = [cotangent(500, 96, dtype, seed=k) for k in range(3)]
+    x = base.clone().requires_grad_()
+    plain, = torch.autograd.grad([torch.nn.functional.linear(x, w.to(dtype)) for w in ws], x, deltas)
+    for _ in range(3):
+        x = base.clone().requires_grad_()
+        packed = activations.pack(x)
+        ours, = torch.autograd.grad([activations.linear(x, w, packed=packed) for w in ws], x, deltas)
+        assert torch.equal(ours, plain)

@@ -1,6 +1,6 @@
 """Numerics of the 8-bit checkpoint operators beyond single calls: statistics
-under autocast, long column sums, negative views, and what is left when a wait
-of the weight gradient runs out.
+under autocast, long sums, negative views, infinities, and what is left when a
+wait of the weight gradient runs out.
 
 Tolerances, from the arithmetic: an FP32 chain of n additions of terms of one
 sign is off by at most n * 2^-24 relative; FP64 joins add one rounding to FP32."""
@@ -145,3 +145,45 @@ def test_views_that_stand_for_their_negative(dtype):
     check_weight_gradient(activations.weight_gradient(x, packed), want, packed)
     assert torch.equal(activations.gelu(x), activations.gelu(want))
     assert torch.equal(activations.gelu_backward(x, packed), activations.gelu_backward(want, packed))
+
+
+# ------------------------------------------------------------------ long sums
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_sums_are_cut_into_chains(dtype):
+    """Tensor cores truncate as they add, so their error grows with the length
+    of a chain; the kernel ends chains after 128 steps (2048 tokens, or 672 for
+    the three products of an FP32 cotangent) and adds them with rounding.  A
+    whole tile of a long sum is therefore, bit for bit, the FP32 sum of what
+    the chains' tokens give on their own.  (Of the 81 tiles the first few are
+    shared out by tokens instead.)"""
+    chain, chains, width = 672 if dtype == torch.float32 else 2048, 8, 2304
+    rows = chain * chains
+    x, delta = activation(rows, width, dtype), cotangent(rows, width, dtype)
+    got = activations.weight_gradient(delta, activations.pack(x))
+    want = 0
+    for i in range(0, rows, chain):
+        want = want + activations.weight_gradient(delta[i:i + chain], activations.pack(x[i:i + chain]))
+    assert torch.equal(got[1024:], want[1024:])
+
+
+# ------------------------------------------------------------------ infinities
+
+@pytest.mark.parametrize("approximate", ["none", "tanh"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [64, 33])
+def test_gelu_of_infinities(cols, dtype, approximate):
+    """+inf gives inf and -inf NaN, as x Phi(x) does in floating point and
+    torch's own GELU; their group's derivative is NaN, and no other's."""
+    x = activation(6, cols, dtype)
+    x[1, 3], x[2, 5] = float("inf"), float("-inf")
+    leaf = x.clone().requires_grad_()
+    y, packed = activations.gelu(leaf, approximate=approximate, pack_output=True)
+    ours, torchs = f64(y), f64(torch.nn.functional.gelu(x, approximate=approximate))
+    assert np.array_equal(np.isnan(ours), np.isnan(torchs)) and np.array_equal(np.isinf(ours), np.isinf(torchs))
+    assert ours[1, 3] == np.inf and np.isnan(ours[2, 5]) and np.isfinite(np.delete(ours, [1, 2], 0)).all()
+    hat = f64(packed.unpack(torch.float32))
+    dx = f64(torch.autograd.grad(y, leaf, torch.ones_like(y))[0])
+    for got in (hat, dx):
+        assert np.isnan(got[1:3, :32]).all() and np.isfinite(got[1:3, 32:]).all()
+        assert np.isfinite(np.delete(got, [1, 2], 0)).all()
