@@ -171,7 +171,7 @@ Packed pack_rows(const Tensor& x, bool stats) {
   return {values, codes, sums};
 }
 
-Packed pack(const Tensor& x, bool stats) {
+Packed pack_values(const Tensor& x, bool stats) {
   no_trace();
   return pack_rows(flat(x.detach(), "an activation"), stats);
 }
@@ -279,26 +279,45 @@ Tensor gelu_backward(const Tensor& delta, const Tensor& values, const Tensor& co
               {delta.requires_grad()})[0];
 }
 
+// Where 16-bit layers that share a checkpoint send their input gradients: a
+// tensor of x's shape in FP32 (one element of memory, never read) whose gradient
+// is x's.  Autograd adds what the layers return for it in FP32, and the sum is
+// rounded to x's type once.
+struct Widen : torch::autograd::Function<Widen> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x) {
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["type"] = static_cast<int64_t>(x.scalar_type());
+    return at::empty({}, x.options().dtype(at::kFloat)).expand(x.sizes());
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return grads;
+    return {grads[0].to(static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()))};
+  }
+};
+
 struct Linear : torch::autograd::Function<Linear> {
+  // x: the input, or where `data` is given its wide stand-in
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const optional<Tensor>& bias,
-                        const Tensor& values, const Tensor& codes) {
-    const at::ScalarType dtype = x.scalar_type();
+                        const Tensor& values, const Tensor& codes, const optional<Tensor>& data) {
+    const Tensor& input = data ? *data : x;
+    const at::ScalarType dtype = input.scalar_type();
     const Tensor cast = weight.to(dtype);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({cast, values, codes});
     ctx->saved_data["weight"] = static_cast<int64_t>(weight.scalar_type());
     ctx->saved_data["bias"] = static_cast<int64_t>(bias ? bias->scalar_type() : at::kFloat);
-    ctx->saved_data["shape"] = x.sizes();
+    ctx->saved_data["shape"] = input.sizes();
     ctx->saved_data["x_grad"] = x.requires_grad();
+    ctx->saved_data["wide"] = data.has_value();
     optional<Tensor> b;
     if (bias) b = bias->to(dtype);
     // a view would not let in-place operations (an activation, a residual) at it
-    const Tensor y = at::linear(x, cast, b);
+    const Tensor y = at::linear(input, cast, b);
     return y.is_view() ? at::_unsafe_view(y, y.sizes()) : y;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list out(5);
+    variable_list out(6);
     if (!grads[0].defined()) return out;
     const bool delta_grad = grads[0].requires_grad();
     {
@@ -306,7 +325,9 @@ struct Linear : torch::autograd::Function<Linear> {
       const variable_list saved = ctx->get_saved_variables();
       const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
       const Tensor rows = flat(grads[0], "a cotangent");
-      if (ctx->needs_input_grad(0)) out[0] = as_shape(at::mm(rows, saved[0]), shape);
+      if (ctx->needs_input_grad(0))
+        out[0] = as_shape(ctx->saved_data["wide"].toBool() ? at::mm(rows, saved[0], at::kFloat) : at::mm(rows, saved[0]),
+                          shape);
       if (ctx->needs_input_grad(1))
         out[1] = weight_gradient_rows(rows, saved[1], saved[2], shape.back(),
                                       static_cast<at::ScalarType>(ctx->saved_data["weight"].toInt()));
@@ -314,7 +335,8 @@ struct Linear : torch::autograd::Function<Linear> {
         out[2] = column_sums(rows).to(static_cast<at::ScalarType>(ctx->saved_data["bias"].toInt()));
     }
     // delta W (W has a gradient, or this node would not be), delta^T x^, sum delta
-    return once(std::move(out), {true, delta_grad || ctx->saved_data["x_grad"].toBool(), delta_grad, false, false});
+    return once(std::move(out),
+                {true, delta_grad || ctx->saved_data["x_grad"].toBool(), delta_grad, false, false, false});
   }
 };
 
@@ -322,19 +344,36 @@ at::ScalarType compute_type(const Tensor& x) {
   return at::autocast::is_autocast_enabled(at::kCUDA) ? at::autocast::get_autocast_dtype(at::kCUDA) : x.scalar_type();
 }
 
-// and whether it is of float16 values.  The sums are always those of x itself:
-// where it was rounded to float16 they take a read of their own.
-std::tuple<Packed, bool> pack_input(const Tensor& x, bool stats) {
-  const bool half = compute_type(x) == at::kHalf;
-  const bool rounded = half && x.scalar_type() != at::kHalf;
-  Packed p = pack(rounded ? x.detach().to(at::kHalf) : x, stats && !rounded);
-  if (stats && rounded) std::get<2>(p) = column_statistics(flat(x.detach(), "an activation"), "an activation");
-  return {p, half};
+// The stand-in of x, where 16-bit layers reading x would send it gradients.
+optional<Tensor> widened(const Tensor& x) {
+  if (!at::GradMode::is_enabled() || !x.requires_grad() || compute_type(x) == at::kFloat || x._fw_grad(0).defined())
+    return std::nullopt;
+  return Widen::apply(x);
 }
 
-// packed_cols, packed_half: of the given checkpoint (values, codes), if any
+std::tuple<Packed, optional<Tensor>> pack(const Tensor& x, bool stats) {
+  Packed p = pack_values(x, stats);
+  return {std::move(p), widened(x)};
+}
+
+// and whether it is of float16 values.  The sums are always those of x itself:
+// where it was rounded to float16 they take a read of their own.
+std::tuple<Packed, bool> pack_input_values(const Tensor& x, bool stats) {
+  const bool half = compute_type(x) == at::kHalf;
+  const bool rounded = half && x.scalar_type() != at::kHalf;
+  Packed p = pack_values(rounded ? x.detach().to(at::kHalf) : x, stats && !rounded);
+  if (stats && rounded) std::get<2>(p) = column_statistics(flat(x.detach(), "an activation"), "an activation");
+  return {std::move(p), half};
+}
+
+std::tuple<Packed, bool, optional<Tensor>> pack_input(const Tensor& x, bool stats) {
+  auto [p, half] = pack_input_values(x, stats);
+  return {std::move(p), half, widened(x)};
+}
+
+// packed_cols, packed_half, wide: of the given checkpoint (values, codes), if any
 Tensor linear(const Tensor& x, const Tensor& weight, const optional<Tensor>& bias, const optional<Tensor>& values,
-              const optional<Tensor>& codes, int64_t packed_cols, bool packed_half) {
+              const optional<Tensor>& codes, int64_t packed_cols, bool packed_half, const optional<Tensor>& wide) {
   TORCH_CHECK_VALUE(weight.dim() == 2 && x.dim() > 0 && x.size(-1) == weight.size(1), "linear: input ", text(x),
                     " does not fit weight ", text(weight));
   TORCH_CHECK_VALUE(!bias || (bias->dim() == 1 && bias->size(0) == weight.size(0)), "linear: bias ",
@@ -361,9 +400,16 @@ Tensor linear(const Tensor& x, const Tensor& weight, const optional<Tensor>& bia
   no_tangent(x);
   no_tangent(weight);
   if (bias) no_tangent(*bias);
-  if (values) return Linear::apply(x.to(dtype), weight, bias, *values, *codes);
-  const Packed p = std::get<0>(pack_input(x, false));
-  return Linear::apply(x.to(dtype), weight, bias, std::get<0>(p), std::get<1>(p));
+  if (!values) {
+    const Packed p = std::get<0>(pack_input_values(x, false));
+    return Linear::apply(x.to(dtype), weight, bias, std::get<0>(p), std::get<1>(p), optional<Tensor>());
+  }
+  // the stand-in is x's where its gradient goes where x's does (and not, say,
+  // to the tensor that x was copied from)
+  if (wide && dtype != at::kFloat && x.requires_grad() && wide->grad_fn() &&
+      wide->grad_fn()->next_edge(0) == torch::autograd::impl::gradient_edge(x))
+    return Linear::apply(*wide, weight, bias, *values, *codes, optional<Tensor>(x.detach().to(dtype)));
+  return Linear::apply(x.to(dtype), weight, bias, *values, *codes, optional<Tensor>());
 }
 
 struct Gelu : torch::autograd::Function<Gelu> {

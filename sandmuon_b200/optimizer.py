@@ -37,7 +37,7 @@ def _pack_with_sums(module, inputs, keywords):
     x = inputs[0] if inputs else None
     if (module.training and torch.is_grad_enabled() and module.weight.requires_grad and isinstance(x, torch.Tensor)
             and _packed_input(module, inputs, keywords) is None):
-        packed = activations.pack_input(x, stats=True)
+        packed = activations.pack_input(x.detach(), stats=True)  # of this layer alone
         if len(inputs) > 1:  # a None in the checkpoint's place
             return (x, packed, *inputs[2:]), keywords
         return inputs, {**keywords, "packed": packed}

@@ -230,18 +230,107 @@ def test_a_gradient_that_nothing_gives():
 
 # ------------------------------------------------- layers that share an input
 
+def shared_exact(deltas, ws, dtype):
+    """(sum of delta W, sum of |delta| |W|) in FP64."""
+    pairs = [(d.double(), w.detach().to(dtype).double()) for d, w in zip(deltas, ws)]
+    return sum(d @ w for d, w in pairs), sum(d.abs() @ w.abs() for d, w in pairs)
+
+
+def check_shared(got, deltas, ws, dtype, out_dtype=None):
+    """FP32 sums of 3 x 96 terms in any order (library products may truncate: a
+    step of 2^-23 a term, and the joins), then half a step of the result's
+    type."""
+    want, size = shared_exact(deltas, ws, dtype)
+    bound = 300 * 2.0 ** -23 * size + torch.finfo(out_dtype or dtype).eps / 2 * want.abs()
+    assert got.dtype == (out_dtype or dtype)
+    assert bool(((got.double().reshape(want.shape) - want).abs() <= bound).all())
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_layers_that_share_an_input_give_the_input_gradient_of_plain_layers(dtype):
-    """Each layer's input gradient is rounded to the input's type and autograd
-    adds them there: bit for bit what as many plain layers give.  Repeated
-    passes give the same bits."""
+@pytest.mark.parametrize("shape", [(500, 80), (5, 100, 80), (80,), (0, 80)])
+def test_input_gradients_of_layers_that_share_a_checkpoint_are_summed_in_fp32(shape, dtype):
     ws = [weight(96, 80, seed) for seed in range(3)]
-    base = activation(500, 80, dtype)
-    deltas = [cotangent(500, 96, dtype, seed=k) for k in range(3)]
+    rows = 1 if len(shape) == 1 else torch.Size(shape[:-1]).numel()
+    base = activation(max(rows, 1), 80, dtype)[:rows].view(shape)
+    deltas = [cotangent(max(rows, 1), 96, dtype, seed=k)[:rows] for k in range(3)]
+    shaped = [d.view(*shape[:-1], 96) for d in deltas]
     x = base.clone().requires_grad_()
-    plain, = torch.autograd.grad([torch.nn.functional.linear(x, w.to(dtype)) for w in ws], x, deltas)
-    for _ in range(3):
-        x = base.clone().requires_grad_()
-        packed = activations.pack(x)
-        ours, = torch.autograd.grad([activations.linear(x, w, packed=packed) for w in ws], x, deltas)
-        assert torch.equal(ours, plain)
+    packed = activations.pack(x)
+    outs = [activations.linear(x, w, packed=packed) for w in ws]
+    first = torch.autograd.grad(outs, [x, *ws], shaped, retain_graph=True)
+    check_shared(first[0], deltas, ws, dtype)
+    for w, dw, d in zip(ws, first[1:], shaped):
+        assert torch.equal(dw, activations.weight_gradient(d, activations.pack(base)))
+    # again, one layer alone, and through x's own graph
+    assert torch.equal(torch.autograd.grad(outs, x, shaped, retain_graph=True)[0], first[0])
+    check_shared(torch.autograd.grad(outs[1], x, shaped[1])[0], deltas[1:2], ws[1:2], dtype)
+    h = x * 2
+    packed = activations.pack(h)
+    got, = torch.autograd.grad([activations.linear(h, w, packed=packed) for w in ws], h, shaped)
+    assert torch.equal(got, first[0])
+    # a checkpoint kept over several passes
+    packed = activations.pack(x)
+    for _ in range(2):
+        got, = torch.autograd.grad([activations.linear(x, w, packed=packed) for w in ws], x, shaped)
+        assert torch.equal(got, first[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_shared_input_gradients_under_autocast(dtype):
+    """FP32 inputs: the sum is not rounded to the layers' type at all."""
+    ws = [weight(96, 80, seed) for seed in range(3)]
+    x = activation(500, 80, torch.float32).requires_grad_()
+    deltas = [cotangent(500, 96, dtype, seed=k) for k in range(3)]
+    with torch.autocast("cuda", dtype=dtype):
+        packed = activations.pack_input(x, stats=True)
+        outs = [activations.linear(x, w, packed=packed) for w in ws]
+    got, = torch.autograd.grad(outs, x, deltas)
+    check_shared(got, deltas, ws, dtype, torch.float32)
+
+
+def test_a_checkpoint_of_another_tensor_sends_no_gradient_there():
+    """The gradient goes to the x that a layer is called with, whatever its
+    checkpoint was packed from."""
+    dtype = torch.bfloat16
+    w, delta = weight(96, 80), cotangent(500, 96, dtype)
+    base = activation(500, 80, dtype)
+    other = base.clone().requires_grad_()
+    packed = activations.pack(other)
+    for make in (lambda: base.clone().requires_grad_(), lambda: (base / 2).requires_grad_() * 2):
+        x = make()
+        got, elsewhere = torch.autograd.grad(activations.linear(x, w, packed=packed), [x, other], delta,
+                                             allow_unused=True)
+        check_shared(got, [delta], [w], dtype)
+        assert elsewhere is None
+    y = activations.linear(base, w, packed=packed)  # data
+    assert torch.autograd.grad(y, [w, other], delta, allow_unused=True)[1] is None
+    # an input changed in place since: its gradient is scaled on its way
+    h = other * 1
+    packed = activations.pack(h)
+    h *= 0.5
+    got, = torch.autograd.grad(activations.linear(h, w, packed=packed), other, delta)
+    check_shared(got * 2, [delta], [w], dtype)
+    # packed where nothing is recorded
+    with torch.no_grad():
+        packed = activations.pack(other)
+    check_shared(torch.autograd.grad(activations.linear(other, w, packed=packed), other, delta)[0], [delta], [w], dtype)
+
+
+def test_checkpoints_of_graph_tensors_can_be_copied():
+    import copy
+    import pickle
+    x = activation(20, 80, torch.bfloat16).requires_grad_()
+    packed = activations.pack(x * 2, stats=True)
+    for again in (copy.copy(packed), copy.deepcopy(packed), pickle.loads(pickle.dumps(packed))):
+        assert torch.equal(again.values, packed.values) and torch.equal(again.exponents, packed.exponents)
+        assert torch.equal(again.sums, packed.sums) and again.shape == packed.shape and again.dtype == packed.dtype
+        assert torch.equal(again.unpack(), packed.unpack())
+
+
+def test_a_penalty_on_a_shared_input_gradient_raises():
+    x, w = activation(40, 80, torch.bfloat16).requires_grad_(), weight(96, 80)
+    packed = activations.pack(x)
+    y = activations.linear(x, w, packed=packed)
+    g, = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate"):
+        (y.sum() + g.square().sum()).backward()
