@@ -440,12 +440,11 @@ __global__ void __launch_bounds__(32 * kFinishLanes)
 
 // --------------------------------------------------------------- the kernels
 
-// Rows in flight per lane, and CTAs resident on an SM: a launch is one wave of
-// them.
+// Rows in flight per lane, and CTAs per SM of a launch: one wave of them (VEC).
 constexpr int kActUnroll = 4;
 constexpr int kPackCtas = 4, kUnpackCtas = 4, kGeluForwardCtas = 4, kGeluBackwardCtas = 4;
 // The residency asked of the compiler; the strided mapping, bound by its
-// element accesses, is left its registers.
+// element accesses, is left its registers and runs in two waves.
 __host__ __device__ constexpr int resident(bool vec, int ctas) { return vec ? ctas : 2; }
 
 // A VEC lane's walk down its rows: where its next row's 8 elements of each

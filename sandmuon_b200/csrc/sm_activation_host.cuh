@@ -32,9 +32,14 @@ struct ActLaunch {
 constexpr int kSumChain = 128;
 
 // CTAs of 256 threads: strips of up to 256 columns times enough row ranges for
-// one wave of `ctas` CTAs per SM, each range of whole passes.  Up to four
-// passes stay in one range: a second launch to join column sums costs more.
-// `sums`: the launch takes column sums; tall inputs then get more ranges.
+// `ctas` CTAs per SM, each range of whole passes (32 rows by 256 columns).  VEC:
+// one wave.  The strided mapping is resident twice per SM and runs two waves:
+// 16384 x 1023 BF16 in one wave instead packs in 65 us, not 74, but its GELU of
+// 16384 x 1111 FP32 takes 57 us, not 39.
+// `sums`: the launch takes column sums.  Two passes then stay in one range, for
+// which no second launch has to join them (64 x 768: pack 3.6 us against 4.5,
+// GELU 5.9 against 5.7; from three passes on the split is faster: 7.7 against
+// 5.7 for GELU), and tall inputs get more ranges.
 static ActLaunch act_launch(int64_t rows, int64_t cols, bool vec, int sms, int ctas, bool sums) {
   ActLaunch l;
   const int64_t padded = act_lde(cols) * kGroup;
@@ -44,7 +49,7 @@ static ActLaunch act_launch(int64_t rows, int64_t cols, bool vec, int sms, int c
   const int64_t strips = cdiv(padded, int64_t{8} << log_lanes);
   const int64_t per_pass = (kActThreads >> log_lanes) * kActUnroll;
   const int64_t want = std::max<int64_t>(1, static_cast<int64_t>(ctas) * sms / strips);
-  const int64_t most = rows <= 4 * per_pass ? 1 : cdiv(rows, per_pass);
+  const int64_t most = sums && rows <= 2 * per_pass ? 1 : cdiv(rows, per_pass);
   int64_t splits = std::min<int64_t>(std::min(want, most), 65535);
   int64_t rows_per_cta = round_up(cdiv(rows, splits), per_pass);
   if (sums)
