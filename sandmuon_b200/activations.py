@@ -54,10 +54,9 @@ class PackedActivation:
     values: int8 [rows, columns rounded up to 16]; exponents: uint8 [rows,
     groups of 32 columns rounded up to 4], e + 127 (255: the group is NaN);
     shape, dtype: of the activation; sums: float32 [2, columns] (column sums of
-    x^2 and of x) or None.  A checkpoint that was packed while autograd records
-    refers to its input's graph (not to the input), a copy of it does not."""
+    x^2 and of x) or None."""
 
-    __slots__ = ("values", "exponents", "shape", "dtype", "sums", "_wide")
+    __slots__ = ("values", "exponents", "shape", "dtype", "sums", "_shared")
 
     def __init__(self, values: torch.Tensor, exponents: torch.Tensor, shape, dtype: torch.dtype,
                  sums: torch.Tensor | None = None):
@@ -77,23 +76,23 @@ class PackedActivation:
         if sums is not None and (sums.dtype != torch.float32 or sums.shape != (2, cols)):
             raise ValueError(f"sums must be float32 [2, {cols}]")
         self.values, self.exponents, self.shape, self.dtype, self.sums = values, exponents, shape, dtype, sums
-        self._wide = None
+        self._shared = None
 
     @classmethod
-    def _made(cls, parts, shape, dtype: torch.dtype, wide: torch.Tensor | None = None) -> "PackedActivation":
-        """From what the binding returns, which needs no checks.  wide: where
-        layers that share the checkpoint send their input gradients."""
+    def _made(cls, parts, shape, dtype: torch.dtype, shared=None) -> "PackedActivation":
+        """From what the binding returns, which needs no checks.  shared: through
+        which layers called with the checkpoint sum their input gradients."""
         self = object.__new__(cls)
         self.values, self.exponents, self.sums = parts
-        self.shape, self.dtype, self._wide = tuple(shape), dtype, wide
+        self.shape, self.dtype, self._shared = tuple(shape), dtype, shared
         return self
 
-    def __getstate__(self):  # a copy is of the values, not of their place in a graph
+    def __getstate__(self):  # a copy is of the values alone
         return self.values, self.exponents, self.sums, self.shape, self.dtype
 
     def __setstate__(self, state):
         self.values, self.exponents, self.sums, self.shape, self.dtype = state
-        self._wide = None
+        self._shared = None
 
     @property
     def device(self) -> torch.device:
@@ -121,8 +120,8 @@ def pack(x: torch.Tensor, *, stats: bool = False) -> PackedActivation:
     """The 8-bit checkpoint of x [..., columns] (any strides; not
     differentiable).  stats: also return the column sums of x^2 and x
     (PackedActivation.sums), from the same read of x."""
-    parts, wide = _lib.binding().pack(x, stats)
-    return PackedActivation._made(parts, x.shape, x.dtype, wide)
+    parts, shared = _lib.binding().pack(x, stats)
+    return PackedActivation._made(parts, x.shape, x.dtype, shared)
 
 
 def pack_input(x: torch.Tensor, *, stats: bool = False) -> PackedActivation:
@@ -130,8 +129,8 @@ def pack_input(x: torch.Tensor, *, stats: bool = False) -> PackedActivation:
     autocast state: of x as it comes, or of its float16 values where the layers
     compute in float16 (their cotangents then need those).  stats: the column
     sums of x as it comes, as the optimizers' hooks of plain layers take them."""
-    parts, half, wide = _lib.binding().pack_input(x, stats)
-    return PackedActivation._made(parts, x.shape, torch.float16 if half else x.dtype, wide)
+    parts, half, shared = _lib.binding().pack_input(x, stats)
+    return PackedActivation._made(parts, x.shape, torch.float16 if half else x.dtype, shared)
 
 
 def unpack(packed: PackedActivation, dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -164,14 +163,14 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     Computes in x's type, or autocast's where it is on; weight and bias are
     cast to it, and their gradients come in their own types, the weight's
     straight from the FP32 sum.  `packed`: x's checkpoint, where the caller has
-    it already (several layers that read one x share one checkpoint, and where
-    it was packed from x itself their input gradients are summed in FP32 and
-    rounded once); else x is packed here if the weight needs a gradient.
+    it already (several layers that read one x share one checkpoint; where it
+    was packed while x takes a gradient, their input gradients are summed in
+    FP32 and rounded once); else x is packed here if the weight needs a gradient.
     Differentiable once."""
     if packed is None:
         return _lib.binding().linear(x, weight, bias, None, None, 0, False, None)
     return _lib.binding().linear(x, weight, bias, packed.values, packed.exponents, packed.shape[-1],
-                                 packed.dtype == torch.float16, packed._wide)
+                                 packed.dtype == torch.float16, packed._shared)
 
 
 class PackedLinear(nn.Linear):

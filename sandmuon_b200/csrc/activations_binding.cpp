@@ -13,8 +13,11 @@
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
+
+#include <mutex>
 
 #include "sandmuon_b200.h"
 
@@ -282,16 +285,13 @@ Tensor gelu_backward(const Tensor& delta, const Tensor& values, const Tensor& co
 // Where 16-bit layers that share a checkpoint send their input gradients: a
 // tensor of x's shape in FP32 (one element of memory, never read) whose gradient
 // is x's.  Autograd adds what the layers return for it in FP32, and the sum is
-// rounded to x's type once.
-struct Widen : torch::autograd::Function<Widen> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x) {
-    ctx->set_materialize_grads(false);
-    ctx->saved_data["type"] = static_cast<int64_t>(x.scalar_type());
-    return at::empty({}, x.options().dtype(at::kFloat)).expand(x.sizes());
-  }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    if (!grads[0].defined()) return grads;
-    return {grads[0].to(static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()))};
+// rounded to x's type once, by this node.
+struct Widen : torch::autograd::Node {
+  const at::ScalarType type;
+  explicit Widen(const Tensor& x)
+      : torch::autograd::Node({torch::autograd::impl::gradient_edge(x)}), type(x.scalar_type()) {}
+  variable_list apply(variable_list&& grads) override {
+    return {grads[0].defined() ? grads[0].to(type) : Tensor()};
   }
 };
 
@@ -344,17 +344,42 @@ at::ScalarType compute_type(const Tensor& x) {
   return at::autocast::is_autocast_enabled(at::kCUDA) ? at::autocast::get_autocast_dtype(at::kCUDA) : x.scalar_type();
 }
 
-// The stand-in of x, where 16-bit layers reading x would send it gradients.
-optional<Tensor> widened(const Tensor& x) {
-  if (!at::GradMode::is_enabled() || !x.requires_grad() || compute_type(x) == at::kFloat || x._fw_grad(0).defined())
-    return std::nullopt;
-  return Widen::apply(x);
+// What the layers that are called with one checkpoint share: the stand-in of the
+// x that they are called with, for as long as one of them holds it.
+struct Shared {
+  std::mutex mutex;
+  std::weak_ptr<torch::autograd::Node> node;
+
+  // The node's gradient goes where x's does (x is not, say, a copy of what it
+  // was made for), and it runs on this stream: a backward pass that is captured
+  // into a graph must not wait on a stream outside of it.
+  static bool stands_for(torch::autograd::Node& node, const Tensor& x) {
+    const optional<c10::Stream> stream = node.stream();
+    return node.next_edge(0) == torch::autograd::impl::gradient_edge(x) && stream &&
+           *stream == c10::cuda::getCurrentCUDAStream(x.device().index()).unwrap();
+  }
+
+  Tensor wide(const Tensor& x) {
+    const Tensor t = at::empty({}, x.options().dtype(at::kFloat)).expand(x.sizes());
+    const std::lock_guard<std::mutex> lock(mutex);
+    if (const auto known = node.lock(); known && stands_for(*known, x)) {
+      torch::autograd::impl::set_gradient_edge(t, {known, 0});
+    } else {
+      const std::shared_ptr<torch::autograd::Node> made(new Widen(x), torch::autograd::deleteNode);
+      torch::autograd::set_history(t, made);
+      node = made;
+    }
+    return t;
+  }
+};
+using SharedRef = std::shared_ptr<Shared>;
+
+// For an x whose layers would send it gradients.
+SharedRef shared_by(const Tensor& x) {
+  return at::GradMode::is_enabled() && x.requires_grad() ? std::make_shared<Shared>() : nullptr;
 }
 
-std::tuple<Packed, optional<Tensor>> pack(const Tensor& x, bool stats) {
-  Packed p = pack_values(x, stats);
-  return {std::move(p), widened(x)};
-}
+std::tuple<Packed, SharedRef> pack(const Tensor& x, bool stats) { return {pack_values(x, stats), shared_by(x)}; }
 
 // and whether it is of float16 values.  The sums are always those of x itself:
 // where it was rounded to float16 they take a read of their own.
@@ -366,14 +391,14 @@ std::tuple<Packed, bool> pack_input_values(const Tensor& x, bool stats) {
   return {std::move(p), half};
 }
 
-std::tuple<Packed, bool, optional<Tensor>> pack_input(const Tensor& x, bool stats) {
+std::tuple<Packed, bool, SharedRef> pack_input(const Tensor& x, bool stats) {
   auto [p, half] = pack_input_values(x, stats);
-  return {std::move(p), half, widened(x)};
+  return {std::move(p), half, shared_by(x)};
 }
 
-// packed_cols, packed_half, wide: of the given checkpoint (values, codes), if any
+// packed_cols, packed_half, shared: of the given checkpoint (values, codes), if any
 Tensor linear(const Tensor& x, const Tensor& weight, const optional<Tensor>& bias, const optional<Tensor>& values,
-              const optional<Tensor>& codes, int64_t packed_cols, bool packed_half, const optional<Tensor>& wide) {
+              const optional<Tensor>& codes, int64_t packed_cols, bool packed_half, const SharedRef& shared) {
   TORCH_CHECK_VALUE(weight.dim() == 2 && x.dim() > 0 && x.size(-1) == weight.size(1), "linear: input ", text(x),
                     " does not fit weight ", text(weight));
   TORCH_CHECK_VALUE(!bias || (bias->dim() == 1 && bias->size(0) == weight.size(0)), "linear: bias ",
@@ -404,11 +429,8 @@ Tensor linear(const Tensor& x, const Tensor& weight, const optional<Tensor>& bia
     const Packed p = std::get<0>(pack_input_values(x, false));
     return Linear::apply(x.to(dtype), weight, bias, std::get<0>(p), std::get<1>(p), optional<Tensor>());
   }
-  // the stand-in is x's where its gradient goes where x's does (and not, say,
-  // to the tensor that x was copied from)
-  if (wide && dtype != at::kFloat && x.requires_grad() && wide->grad_fn() &&
-      wide->grad_fn()->next_edge(0) == torch::autograd::impl::gradient_edge(x))
-    return Linear::apply(*wide, weight, bias, *values, *codes, optional<Tensor>(x.detach().to(dtype)));
+  if (shared && dtype != at::kFloat && x.requires_grad())
+    return Linear::apply(shared->wide(x), weight, bias, *values, *codes, optional<Tensor>(x.detach().to(dtype)));
   return Linear::apply(x.to(dtype), weight, bias, *values, *codes, optional<Tensor>());
 }
 
@@ -466,6 +488,7 @@ std::tuple<Tensor, optional<Packed>> gelu(const Tensor& x, int64_t form, bool pa
 using Unlocked = pybind11::call_guard<pybind11::gil_scoped_release>;
 
 PYBIND11_MODULE(_activations, m) {
+  pybind11::class_<Shared, SharedRef>(m, "Shared");
   m.def("bind", &bind);
   m.def("pack", &pack, Unlocked());
   m.def("pack_input", &pack_input, Unlocked());

@@ -334,3 +334,59 @@ def test_a_penalty_on_a_shared_input_gradient_raises():
     g, = torch.autograd.grad(y.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="differentiate"):
         (y.sum() + g.square().sum()).backward()
+
+
+CAPTURED = """
+import torch
+from sandmuon_b200 import activations
+g = torch.Generator(device="cuda").manual_seed(1)
+x = torch.randn(300, 80, generator=g, device="cuda").bfloat16().requires_grad_()
+ws = [torch.randn(96, 80, generator=g, device="cuda").mul_(.05).requires_grad_() for _ in range(2)]
+d = torch.randn(300, 96, generator=g, device="cuda").bfloat16()
+
+def work(packed=None):
+    packed = packed or activations.pack(x)
+    outs = [activations.linear(x, w, packed=packed) for w in ws]
+    y, py = activations.gelu(x, pack_output=True)
+    return torch.autograd.grad([*outs, y], [x, *ws], [d, d, x.detach()])
+
+want = work()
+kept = activations.pack(x)  # on another stream than the capture's
+[activations.linear(x, w, packed=kept) for w in ws]
+for packed in (None, kept):
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work(packed)
+    for t in got:
+        t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+print("ok")
+"""
+
+
+def test_a_captured_backward_with_a_checkpoint_from_outside():
+    """In a process of its own, which a failed capture would leave unusable.
+    (An eager graph of the same leaves must not live meanwhile, with torch's own
+    layers neither.)"""
+    import subprocess
+    import sys
+    from pathlib import Path
+    out = subprocess.run([sys.executable, "-c", CAPTURED], capture_output=True, text=True, timeout=300,
+                         cwd=Path(__file__).resolve().parents[1])
+    assert out.returncode == 0 and out.stdout.strip().endswith("ok"), out.stderr[-2000:]
+
+
+def test_a_kept_checkpoint_keeps_no_graph_alive():
+    x = activation(1024, 1024, torch.bfloat16).requires_grad_()
+    w = weight(96, 1024)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    h = x.exp().exp()  # keeps two results for its backward
+    packed = activations.pack(h)
+    outs = [activations.linear(h, w, packed=packed) for _ in range(2)]
+    assert torch.autograd.grad(outs, x, [torch.ones_like(y) for y in outs], retain_graph=True)[0].shape == x.shape
+    del h, outs
+    assert torch.cuda.memory_allocated() - before <= packed.nbytes + 4096
