@@ -14,7 +14,9 @@
 // stride), padding 0; codes e + 127 [rows, lde] uint8, lde = groups rounded up
 // to 4, padding 127 (scale 1).
 //
-// All kernels here read and write each element once and are bound by HBM.
+// All kernels here read and write each element once.  Packing and unpacking of
+// aligned rows are bound by HBM, the strided mapping by its element accesses and
+// GELU by load latency and instruction issue together (see there).
 // Two mappings of a warp onto a row:
 //   VEC   a lane owns 8 consecutive columns (16- or 32-byte accesses, 4 lanes
 //         share a group's maximum by two shuffles); needs cols % 8 == 0 and
@@ -65,8 +67,9 @@ template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
 // Two FP32 values in one 64-bit register pair, for the packed instructions of
-// sm_100: these kernels are bound by instruction issue, and one packed
-// instruction does two elements' work with the same roundings.
+// sm_100: one packed instruction takes one issue slot for two elements' work,
+// with the same roundings (GELU of 16384 x 4096 BF16: forward 107 -> 99 us,
+// backward 76 -> 60 us).
 struct Pair {
   uint64_t v;
   __device__ __forceinline__ Pair() {}
@@ -566,16 +569,21 @@ __global__ void __launch_bounds__(kActThreads, resident(VEC, kUnpackCtas))
 
 // ---------------------------------------------------------------------- GELU
 //
-// gelu(x) = x Phi(x).  With h = Phi(-|x|):  gelu = max(x, 0) - |x| h, which
-// keeps the relative accuracy of the negative tail.  h = exp(-x^2/2) u G(u),
+// gelu(x) = x Phi(x).  With h = Phi(-|x|):  gelu = max(x, 0) - |x| h, in which
+// the negative tail does not cancel.  h = exp(-x^2/2) u G(u),
 // u = 1 / (1 + p |x|): exp(x^2/2) Phi(-|x|) is smooth in u down to u = 0, and a
-// polynomial of degree 8 holds it within 3e-8 relative over |x| < 14.5, where
-// Phi(-|x|) leaves FP32 (3.2e-7 with FP32 coefficients and roundings).  The
+// polynomial of degree 8 holds it within 3e-8 relative over |x| < 14.5 (3.2e-7
+// with FP32 coefficients and roundings).  The exponential adds the rounding of
+// its argument, x^2 / 2: measured against FP64, gelu is within 4e-7 relative
+// for -1 < x, 1.3e-6 to -5, 4.9e-6 to -10 and 8.8e-6 to -13.2; below, the
+// exponential underflows and gelu is 0 (true values under 5e-39).  The
 // coefficients are a minimax fit (iteratively reweighted least squares on
 // Chebyshev nodes) to exp(x^2/2) erfc(|x|/sqrt 2) / (2 u).  The same
 // exponential gives the density phi(x) of the derivative Phi(x) + x phi(x).
 // CUDA's erfcf instead of this: 241 us forward, 187 us backward for
-// 16384 x 4096 BF16.
+// 16384 x 4096 BF16, where this takes 98 and 60 (floors 62 and 51.5).  The
+// forward pass issues in 63% of its cycles and stalls first for its loads, two
+// rows of which are in flight per lane; the backward pass issues in 70%.
 
 __device__ __forceinline__ float ex2_approx(float v) {
   float r;
