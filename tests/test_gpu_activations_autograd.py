@@ -288,6 +288,25 @@ def test_shared_input_gradients_under_autocast(dtype):
     check_shared(got, deltas, ws, dtype, torch.float32)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,d_in,d_out", [(7, 33, 5), (257, 129, 1), (1, 1, 1), (40, 24, 0), (64, 8, 1000)])
+def test_shared_input_gradients_of_odd_sizes_and_strides(rows, d_in, d_out, dtype):
+    """Weights and cotangents of any strides (a transposed weight, a broadcast
+    cotangent), sizes without alignment, a layer without outputs."""
+    x = activation(rows, d_in, dtype).requires_grad_()
+    base = weight(d_in, d_out, 1).detach()
+    ws = [base.t().requires_grad_(), weight(d_out, d_in, 2)]
+    deltas = [cotangent(rows, d_out, dtype), cotangent(rows, 1, dtype).expand(rows, d_out)]
+    packed = activations.pack(x)
+    outs = [activations.linear(x, w, packed=packed) for w in ws]
+    got = torch.autograd.grad(outs, [x, *ws], deltas)
+    want, size = shared_exact(deltas, ws, dtype)
+    bound = (2 * d_out + 20) * 2.0 ** -23 * size + torch.finfo(dtype).eps / 2 * want.abs()
+    assert bool(((got[0].double() - want).abs() <= bound + torch.finfo(dtype).smallest_normal).all())
+    for dw, d in zip(got[1:], deltas):
+        assert torch.equal(dw, activations.weight_gradient(d, packed))
+
+
 def test_a_checkpoint_of_another_tensor_sends_no_gradient_there():
     """The gradient goes to the x that a layer is called with, whatever its
     checkpoint was packed from."""

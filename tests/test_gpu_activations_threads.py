@@ -85,4 +85,4 @@ def test_a_call_that_waits_for_the_launch_queue_holds_no_python_lock():
         thread.join()
         torch.cuda.synchronize()
     assert longest > 0.1, "the launch queue never filled up"
-    assert max(gaps) < longest / 2
+    assert max(gaps) < 0.8 * longest
